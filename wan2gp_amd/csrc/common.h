@@ -70,6 +70,12 @@ __device__ __forceinline__ uint16_t f2h(float f) { return __builtin_bit_cast(uin
 // element-type dispatch for kernels templated on the 16-bit storage type (bf16 DiT / fp16 VAE)
 template <bool F16> __device__ __forceinline__ float ld16(uint16_t v) { return F16 ? h2f(v) : bf2f(v); }
 template <bool F16> __device__ __forceinline__ uint16_t st16(float f) { return F16 ? f2h(f) : f2bf(f); }
+// An fp32 result that is rounded to fp16 afterwards: held in a register, so that hipcc does not fold the multiply-add and the rounding into one
+// v_fma_mixlo_f16 (which rounds once where fp32 accumulation and an fp16 store round twice: other bits)
+template <bool F16> __device__ __forceinline__ float hold32(float f) {
+  if (F16) asm volatile("" : "+v"(f));
+  return f;
+}
 template <bool F16> __device__ __forceinline__ float rnd16(float f) { return ld16<F16>(st16<F16>(f)); }
 template <bool F16> __device__ __forceinline__ void unpack8t(const uint4& v, float* f);
 template <bool F16> __device__ __forceinline__ uint4 pack8t(const float* f);

@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void gemm256k_kernel(const bf16_t* __restrict_
       const f32x16 av = acc[yt][xt];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        v[r] = av[r] * out_scale + (BIAS_ROWS ? brow : bcol[r]);
+        v[r] = hold32<F16>(av[r] * out_scale + (BIAS_ROWS ? brow : bcol[r]));
         // nn.Linear output is a 16-bit tensor: GELU sees the rounded value; otherwise the pack below is that rounding
         if (EPI == WAN_EPI_GELU_TANH) v[r] = g256k_gelu_tanh(rnd16<F16>(v[r]));
       }

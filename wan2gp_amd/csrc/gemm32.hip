@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void gemm32_kernel(const bf16_t* __restrict
       const f32x16 av = acc[yt][xt];
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        v[r] = rnd16<F16>(av[r] * out_scale + (BIAS_ROWS ? brow : bcol[r]));  // nn.Linear output is a 16-bit tensor
+        v[r] = rnd16<F16>(hold32<F16>(av[r] * out_scale + (BIAS_ROWS ? brow : bcol[r])));  // nn.Linear output is a 16-bit tensor
       bf16_t* optr = Out + yr * ldo + xb;
       if (xb + 16 <= XN) {
         if (EPI == WAN_EPI_GELU_TANH) {

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void gemm_bf16_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float b = BIAS_ROWS ? brow : bcol[xt * 4 + r];
-        v[xt * 4 + r] = rnd16<F16>(acc[yt][xt][r] * out_scale + b);  // nn.Linear output is a 16-bit tensor
+        v[xt * 4 + r] = rnd16<F16>(hold32<F16>(acc[yt][xt][r] * out_scale + b));  // nn.Linear output is a 16-bit tensor
       }
     bf16_t* optr = Out + yr * ldo + xb;
     if (xb + 16 <= XN) {
