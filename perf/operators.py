@@ -112,7 +112,7 @@ def _weight(g, N, K):
     """A weight quantised at load: codes [N, K / 2] and scales in the kernels' order."""
     w = torch.randn(N, K, generator=g, device="cuda", dtype=F32) * (1.0 / math.sqrt(K))
     codes, exps = _encode(w.to(BF16))
-    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).contiguous(), _tile(exps)
+    return (codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8).contiguous(), _tile(exps)
 
 
 def prepare(case, seed):
