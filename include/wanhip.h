@@ -148,6 +148,27 @@ int wan_gemm_fp8_amax(const uint8_t* A, int64_t lda, const float* scale_a, const
                       const wan_bf16* bias, wan_bf16* C, int64_t M, int N, int K, float* amax, void* stream);
 int wan_fp8_quantize_pre(const wan_bf16* x, uint8_t* out, float* ws, int64_t n, int amax_word, void* stream);
 
+/* ---- MXFP4 Linear: 4-bit floating point with one power of two per 32 values (OCP MX) ------------------------------------
+ * codes  [rows][K / 2] bytes: e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), the even element in the low nibble.
+ * scales e8m0 bytes (2^(byte - 127), 255 = NaN), one per 32 consecutive values of a row, in the order of the matrix instruction's lanes:
+ *        tiles of 128 rows x 8 blocks (256 values), 1,024 bytes each, row tiles outside; the byte of row r, block j of a tile at
+ *        [j & 3][r >> 3][j >> 2][r & 7]; bytes past the matrix are 0.  wan_mxfp4_scale_bytes(rows, K) bytes.
+ * wan_mxfp4_quantize: x [M, K] bf16 (rows row_stride elements apart) -> codes, scales.  Exponent of a block: floor(log2 amax) - 2, one more
+ *   where amax >= 1.75 of its power of two, kept in [-127, 125]; elements to nearest even, at most 6.  A block with an inf or a NaN: NaN.
+ * wan_mxfp4_dequantize: the values that the codes stand for, bf16 [M, K] (exact).
+ * wan_gemm_mxfp4: C = epilogue(A W^T + bias), A [M, K] and W [N, K] quantised, C bf16; epilogues and their arguments as wan_gemm_bf16 (the
+ *   transposed form writes Ct [N, ldc]).  K % 32 == 0, any M and N.  The whole epilogue in fp32, ONE rounding to bf16 at its end (no
+ *   reference plan fixes roundings in between, and each would cost a bit).  scratch: wan_gemm_mxfp4_scratch_bytes(M, N, K, epilogue) bytes of device memory, 16-byte aligned
+ *   (NULL where that is 0); a call overwrites it, calls on different streams must not share it. */
+int64_t wan_mxfp4_scale_bytes(int64_t rows, int64_t K);
+int wan_mxfp4_quantize(const wan_bf16* x, int64_t row_stride, uint8_t* codes, uint8_t* scales, int64_t M, int K, void* stream);
+int wan_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, wan_bf16* out, int64_t M, int K, void* stream);
+int64_t wan_gemm_mxfp4_scratch_bytes(int64_t M, int N, int K, int epilogue);
+int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias,
+                   wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue, const wan_bf16* R, const wan_bf16* mod,
+                   const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes,
+                   void* stream);
+
 /* ---- attention ------------------------------------------------------------------------- */
 
 /* Exact (non-causal, unmasked) flash attention, bf16 in/out, fp32 softmax/accumulate,
@@ -210,6 +231,30 @@ int wan_attention_sp_local(const wan_bf16* q, const wan_bf16* k_local, const wan
 int wan_attention_sp_remote(const wan_bf16* q, const wan_bf16* k_all, const wan_bf16* vt_all, wan_bf16* o, int B, int64_t Lq,
                             int64_t Lk, int64_t ldv, int H, int nseg, int64_t k_seg_stride, int64_t vt_seg_stride, int own_seg,
                             float* scratch, float* raw, void* stream);
+/* ---- block-sparse attention: each block of 128 queries attends its own list of blocks of 64 keys ---------------------------
+ * wan_block_mean: x [B, L, H, 128] bf16 (rows row_stride, batches batch_stride elements apart) -> out [B, H, ceil(L / block), 128] fp32, the
+ *   mean of each block's rows below lens[b] (device int32 [B] or NULL = L; values outside [0, L] count as the nearest); 0 where a block has none.
+ * wan_select_blocks: q_mean [B, H, nq, 128], k_mean [Bk, Hk, nk, 128] -> index [B, H, nq, keep]: the blocks of keys with the `keep` largest
+ *   products q_mean . k_mean (summed in 64 bits; equal ones: the lowest first; NaN above everything), ascending, -1 behind the last;
+ *   count [B, H, nq]: how many there are.  Only the first ceil(k_lens[b] / 64) blocks are candidates (k_lens: device int32 [Bk] or NULL = all).
+ *   Query batch b reads k batch b mod Bk, query head h k head h / (H / Hk).  nk <= 20,000.  scratch: wan_select_blocks_scratch_bytes(...).
+ * wan_sparse_attention: softmax(q k^T / sqrt(128)) v over the keys of the listed blocks that lie below k_lens[b].  q [B, Lq, H, 128],
+ *   k [Bk, Lk, Hk, 128] (rows / batches q_row, q_batch, k_row, k_batch elements apart), vt [Bk, Hk * 128, ldv] as wan_attention takes it
+ *   (columns past k_lens may hold anything), o [B, Lq, H, 128] contiguous (may be q, where q is contiguous).  index / count as
+ *   wan_select_blocks leaves them, in any order; entries outside [0, ceil(k_lens / 64)) are skipped, a block listed twice counts twice;
+ *   count NULL = all `keep` entries.  A query without a key gets zeros.  q_prescaled: q already holds q * wan_attention_qscale().
+ *   scratch: wan_sparse_attention_scratch_bytes(...) bytes of device memory, 16-byte aligned (NULL where that is 0); a call overwrites it,
+ *   calls on different streams must not share it. */
+int wan_block_mean(const wan_bf16* x, int64_t row_stride, int64_t batch_stride, const int* lens, float* out, int B, int64_t L, int H,
+                   int block, void* stream);
+int64_t wan_select_blocks_scratch_bytes(int B, int H, int64_t nq, int64_t nk);
+int wan_select_blocks(const float* q_mean, const float* k_mean, const int* k_lens, int* index, int* count, int B, int Bk, int H, int Hk,
+                      int64_t nq, int64_t nk, int keep, void* scratch, int64_t scratch_bytes, void* stream);
+int64_t wan_sparse_attention_scratch_bytes(int B, int64_t Lq, int H, int keep);
+int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_batch, const wan_bf16* k, int64_t k_row, int64_t k_batch,
+                         const wan_bf16* vt, wan_bf16* o, const int* index, const int* count, const int* k_lens, int B, int Bk, int64_t Lq,
+                         int64_t Lk, int64_t ldv, int H, int Hk, int keep, int q_prescaled, void* scratch, int64_t scratch_bytes,
+                         void* stream);
 /* (1/sqrt(128)) * log2(e): the factor wan_attention_prescaled expects folded into q */
 float wan_attention_qscale(void);
 

@@ -96,6 +96,19 @@ SIGNATURES = {
     "wan_attention_sp_remote": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int64,
                                         c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "wan_attention_qscale": (c_float, []),
+    "wan_mxfp4_scale_bytes": (c_int64, [c_int64, c_int64]),
+    "wan_mxfp4_quantize": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "wan_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
+    "wan_gemm_mxfp4_scratch_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "wan_gemm_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
+                               c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_int64, c_void_p]),
+    "wan_block_mean": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p]),
+    "wan_select_blocks_scratch_bytes": (c_int64, [c_int, c_int, c_int64, c_int64]),
+    "wan_select_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int,
+                                  c_void_p, c_int64, c_void_p]),
+    "wan_sparse_attention_scratch_bytes": (c_int64, [c_int, c_int64, c_int, c_int]),
+    "wan_sparse_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "wan_transpose_v": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
     "wan_t5_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "wan_mul_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),

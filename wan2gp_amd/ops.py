@@ -323,6 +323,218 @@ def attention_sp(q, k_local, vt_local, k_all, vt_all, own_seg, out=None):
     return out, scratch
 
 
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise _L.WanHipError(f"all tensors must be on one device, got {first.device} and {t.device}")
+
+
+def _token_strides(t, name):
+    """(row, batch) strides in elements of a bf16 [B, L, H, 128] tensor whose heads lie side by side in a row: a slice of a fused projection
+    is taken as it is."""
+    if not t.is_cuda:
+        raise _L.WanHipError(f"{name} must be a CUDA(HIP) tensor -- libwanhip has no CPU path")
+    if t.dtype != BF16:
+        raise _L.WanHipError(f"{name} must be {BF16}, got {t.dtype}")
+    if t.dim() != 4 or t.shape[3] != 128:
+        raise _L.WanHipError(f"{name} must be [B, L, H, 128], got {list(t.shape)}")
+    B, L, H, _ = t.shape
+    if t.stride(3) != 1 or (H > 1 and t.stride(2) != 128):
+        raise _L.WanHipError(f"{name}: the heads of a row must be contiguous")
+    row = t.stride(1) if L > 1 else H * 128
+    return row, (t.stride(0) if B > 1 else L * row)
+
+
+def _lens(t, n, name, device):
+    if t is None:
+        return
+    _req(t, torch.int32, name)
+    if t.numel() != n:
+        raise _L.WanHipError(f"{name} must hold {n} lengths, got {t.numel()}")
+    if t.device != device:
+        raise _L.WanHipError(f"{name} must be on {device}")
+
+
+def block_mean(x, block, lens=None):
+    """Mean of each block of `block` tokens of x [B,L,H,128] bf16 (rows may be strided) -> fp32 [B,H,ceil(L/block),128].  lens: int32 [B] on the
+    device, tokens from there on are left out (a block without any: 0).  Sums in 64 bits."""
+    row, batch = _token_strides(x, "x")
+    B, L, H, _ = x.shape
+    _lens(lens, B, "lens", x.device)
+    if block < 1:
+        raise _L.WanHipError("block must be positive")
+    out = torch.empty(B, H, (L + block - 1) // block, 128, dtype=torch.float32, device=x.device)
+    if out.numel():
+        with torch.cuda.device(x.device):
+            check(_L.load().wan_block_mean(ptr(x), row, batch, ptr(lens), ptr(out), B, L, H, block, stream_ptr()), "wan_block_mean")
+    return out
+
+
+def select_blocks(q_mean, k_mean, keep, k_lens=None):
+    """The `keep` blocks of 64 keys with the largest q_mean . k_mean of every block of queries (64-bit sums; equal scores: the lowest block): q_mean
+    [B,H,nq,128], k_mean [Bk,Hk,nk,128] fp32 (block_mean(q, 128), block_mean(k, 64, k_lens)) -> (index int32 [B,H,nq,keep] ascending, -1 behind
+    the last; count int32 [B,H,nq]).  k_lens: int32 [Bk] on the device, blocks past them are no candidates."""
+    _req(q_mean, torch.float32, "q_mean"); _req(k_mean, torch.float32, "k_mean")
+    if q_mean.dim() != 4 or k_mean.dim() != 4 or q_mean.shape[3] != 128 or k_mean.shape[3] != 128:
+        raise _L.WanHipError(f"the means must be [B, H, blocks, 128], got {list(q_mean.shape)} and {list(k_mean.shape)}")
+    B, H, nq, _ = q_mean.shape
+    Bk, Hk, nk, _ = k_mean.shape
+    _same_device(q_mean, k_mean)
+    _lens(k_lens, Bk, "k_lens", q_mean.device)
+    index = torch.empty(B, H, nq, keep, dtype=torch.int32, device=q_mean.device)
+    count = torch.empty(B, H, nq, dtype=torch.int32, device=q_mean.device)
+    if nk == 0 and k_mean.shape[0] and keep > 0:
+        return index.fill_(-1), count.zero_()
+    if nq == 0 and B and H and keep > 0:
+        return index, count
+    lib = _L.load()
+    need = int(lib.wan_select_blocks_scratch_bytes(B, H, nq, nk))
+    with torch.cuda.device(q_mean.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device)
+        check(lib.wan_select_blocks(ptr(q_mean), ptr(k_mean), ptr(k_lens), ptr(index), ptr(count), B, Bk, H, Hk, nq, nk, keep, ptr(ws), need, stream_ptr()),
+              "wan_select_blocks")
+    return index, count
+
+
+def sparse_attention(q, k, vt, block_index, block_count=None, k_lens=None, out=None, q_prescaled=False):
+    """softmax(q k^T / sqrt(128)) v over the listed blocks of 64 keys, v given transposed: q [B,Lq,H,128], k [Bk,Lk,Hk,128] (rows may be strided; Bk divides
+    B, Hk divides H), vt [Bk,Hk*128,ldv]; block_index int32 [B,H,ceil(Lq/128),keep], block_count int32 [B,H,ceil(Lq/128)] or None (all entries) as
+    select_blocks returns them.  k_lens: int32 [Bk] on the device, keys from there on are not attended, whatever they hold.  Entries that name no
+    block are skipped; a query without a key gets zeros.  q_prescaled: q already holds q * attention_qscale().  out may be a contiguous q."""
+    q_row, q_batch = _token_strides(q, "q")
+    k_row, k_batch = _token_strides(k, "k")
+    _req(vt, BF16, "vt"); _req(block_index, torch.int32, "block_index"); _req(block_count, torch.int32, "block_count"); _req(out, BF16, "out")
+    B, Lq, H, _ = q.shape
+    Bk, Lk, Hk, _ = k.shape
+    _same_device(q, k, vt, block_index, block_count, out)
+    _lens(k_lens, Bk, "k_lens", q.device)
+    nq = (Lq + 127) // 128
+    if block_index.dim() != 4 or tuple(block_index.shape[:3]) != (B, H, nq):
+        raise _L.WanHipError(f"block_index must be [{B}, {H}, {nq}, keep], got {list(block_index.shape)}")
+    if block_count is not None and tuple(block_count.shape) != (B, H, nq):
+        raise _L.WanHipError(f"block_count must be [{B}, {H}, {nq}], got {list(block_count.shape)}")
+    if vt.dim() != 3 or vt.shape[0] != Bk or vt.shape[1] != Hk * 128:
+        raise _L.WanHipError(f"vt must be [{Bk}, {Hk * 128}, ldv], got {list(vt.shape)}")
+    if out is not None and out.shape != q.shape:
+        raise _L.WanHipError(f"out must be {list(q.shape)}, got {list(out.shape)}")
+    keep, ldv = block_index.shape[3], vt.shape[2]
+    out = torch.empty(B, Lq, H, 128, dtype=BF16, device=q.device) if out is None else out
+    if Lq == 0 or B == 0:
+        return out
+    if Lk == 0 or keep == 0:
+        return out.zero_()
+    lib = _L.load()
+    need = int(lib.wan_sparse_attention_scratch_bytes(B, Lq, H, keep))
+    with torch.cuda.device(q.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        check(lib.wan_sparse_attention(ptr(q), q_row, q_batch, ptr(k), k_row, k_batch, ptr(vt), ptr(out), ptr(block_index), ptr(block_count), ptr(k_lens), B, Bk, Lq, Lk,
+                                       ldv, H, Hk, keep, 1 if q_prescaled else 0, ptr(ws), need, stream_ptr()), "wan_sparse_attention")
+    return out
+
+
+def mxfp4_quantize(x):
+    """x [..., K] bf16 (rows of a 2-D tensor may be strided) -> (codes uint8 [..., K/2], scales uint8): 4-bit floating point with a power of two per
+    32 values; the layouts are those of include/wanhip.h (the scales in the order of the matrix instruction's lanes)."""
+    if not x.is_cuda:
+        raise _L.WanHipError("x must be a CUDA(HIP) tensor -- libwanhip has no CPU path")
+    if x.dtype != BF16:
+        raise _L.WanHipError(f"x must be {BF16}, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise _L.WanHipError(f"the last dimension of x must be a positive multiple of 32, got {list(x.shape)}")
+    K = x.shape[-1]
+    M = x.numel() // K
+    if x.is_contiguous():
+        row = K
+    elif x.dim() == 2 and x.stride(1) == 1:
+        row = x.stride(0)
+    else:
+        raise _L.WanHipError("x must be contiguous, or 2-D with contiguous rows")
+    lib = _L.load()
+    codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(int(lib.wan_mxfp4_scale_bytes(M, K)), dtype=torch.uint8, device=x.device)
+    if M:
+        with torch.cuda.device(x.device):
+            check(lib.wan_mxfp4_quantize(ptr(x), row, ptr(codes), ptr(scales), M, K, stream_ptr()), "wan_mxfp4_quantize")
+    return codes, scales
+
+
+def _mx_operand(codes, scales, name):
+    _req(codes, torch.uint8, name); _req(scales, torch.uint8, name + " scales")
+    if codes.dim() < 1 or codes.shape[-1] == 0 or codes.shape[-1] % 16:
+        raise _L.WanHipError(f"{name}: the last dimension must be a positive multiple of 16 bytes (32 values), got {list(codes.shape)}")
+    _same_device(codes, scales)
+    K = codes.shape[-1] * 2
+    M = codes.numel() // (K // 2)
+    need = int(_L.load().wan_mxfp4_scale_bytes(M, K))
+    if scales.numel() != need:
+        raise _L.WanHipError(f"{name} scales must hold {need} bytes, got {scales.numel()}")
+    return M, K
+
+
+def mxfp4_dequantize(codes, scales):
+    """The values that mxfp4_quantize's codes stand for, bf16 [..., K] (exact)."""
+    M, K = _mx_operand(codes, scales, "codes")
+    out = torch.empty(*codes.shape[:-1], K, dtype=BF16, device=codes.device)
+    if M:
+        with torch.cuda.device(codes.device):
+            check(_L.load().wan_mxfp4_dequantize(ptr(codes), ptr(scales), ptr(out), M, K, stream_ptr()), "wan_mxfp4_dequantize")
+    return out
+
+
+def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, residual=None, mod=None, e=None, gate_idx=-1, out=None, ldc=None,
+                 x_mx=None):
+    """nn.Linear on MXFP4 operands with an optional fused epilogue (linear's): x [..., K] bf16 is quantised (or pass x_mx = mxfp4_quantize(x) to share
+    it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight)."""
+    for t, n in ((bias, "bias"), (residual, "residual"), (mod, "mod"), (e, "e"), (out, "out")):
+        _req(t, BF16, n)
+    if weight_codes.dim() != 2:
+        raise _L.WanHipError(f"weight_codes must be [N, K / 2], got {list(weight_codes.shape)}")
+    N, K = _mx_operand(weight_codes, weight_scales, "weight_codes")
+    if x_mx is None:
+        if x.shape[-1] != K:
+            raise _L.WanHipError(f"x has rows of {x.shape[-1]} values, the weight of {K}")
+        x_mx = mxfp4_quantize(x)
+    xc, xs = x_mx
+    M, Kx = _mx_operand(xc, xs, "x_mx")
+    if Kx != K:
+        raise _L.WanHipError(f"x has rows of {Kx} values, the weight of {K}")
+    _same_device(xc, weight_codes, bias, residual, mod, e, out)
+    if bias is not None and bias.numel() != N:
+        raise _L.WanHipError(f"bias must hold {N} values")
+    if epilogue == EPI_TRANSPOSED:
+        ldc = ldc or ((M + 63) // 64) * 64
+        if out is None:
+            out = torch.zeros(N, ldc, dtype=BF16, device=xc.device)
+        shape_ok = out.numel() >= N * ldc and ldc >= M
+    else:
+        ldc = N
+        if out is None:
+            out = torch.empty(*xc.shape[:-1], N, dtype=BF16, device=xc.device)
+        shape_ok = out.numel() == M * N
+    if not shape_ok:
+        raise _L.WanHipError(f"out {list(out.shape)} does not hold the result ({M} x {N}, ldc {ldc})")
+    n_mod, nb = 0, 1
+    if epilogue == EPI_GATE_RES:
+        if residual is None or residual.numel() != M * N:
+            raise _L.WanHipError(f"the gated residual needs a residual of {M} x {N} values")
+        if gate_idx >= 0:
+            if mod is None or e is None or mod.numel() % N or gate_idx >= mod.numel() // N or e.numel() == 0 or e.numel() % mod.numel():
+                raise _L.WanHipError("the gate needs mod [.., n_mod, N] with row gate_idx, and e [batches, n_mod, N]")
+            n_mod = mod.numel() // N
+            nb = e.numel() // mod.numel()
+            if M % nb:
+                raise _L.WanHipError(f"{M} rows do not split into {nb} batches")
+    if M == 0:
+        return out
+    lib = _L.load()
+    need = int(lib.wan_gemm_mxfp4_scratch_bytes(M, N, K, epilogue))
+    with torch.cuda.device(xc.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=xc.device) if need else None
+        check(lib.wan_gemm_mxfp4(ptr(xc), ptr(xs), ptr(weight_codes), ptr(weight_scales), ptr(bias), ptr(out), ldc, M, N, K, epilogue, ptr(residual), ptr(mod), ptr(e),
+                                 n_mod, gate_idx, M // nb, ptr(ws), need, stream_ptr()), "wan_gemm_mxfp4")
+    return out
+
+
 def pay_attention(qkv_list, dropout_p=0., softmax_scale=None, causal=False, window_size=(-1, -1),
                   deterministic=False, version=None, force_attention=None, attention_mask=None, recycle_q=False,
                   q_lens=None, k_lens=None):
@@ -341,6 +553,21 @@ def pay_attention(qkv_list, dropout_p=0., softmax_scale=None, causal=False, wind
     q = q.to(BF16).contiguous(); k = k.to(BF16).contiguous(); v = v.to(BF16).contiguous()
     vt = transpose_v(v)
     o = attention(q, k, vt, out=q if (recycle_q and out_dtype == BF16) else None)
+    return o.type(out_dtype)
+
+
+def pay_sparse_attention(qkv_list, keep, k_lens=None, recycle_q=False):
+    """pay_attention with every block of 128 queries attending only the `keep` blocks of 64 keys whose mean key has the largest product with the block's mean
+    query.  Same conventions: q [B,Lq,H,128], k, v [Bk,Lk,Hk,128], the list is consumed, k / v batch 1 is broadcast, the result has q's
+    dtype; recycle_q lets the output reuse q's storage.  k_lens: int32 [Bk] on the device."""
+    q, k, v = qkv_list
+    qkv_list.clear()
+    out_dtype = q.dtype
+    q = q.to(BF16); k = k.to(BF16); v = v.to(BF16).contiguous()
+    if k.shape[1] == 0:
+        return torch.zeros(q.shape, dtype=out_dtype, device=q.device)
+    index, count = select_blocks(block_mean(q, 128), block_mean(k, 64, k_lens), keep, k_lens)
+    o = sparse_attention(q, k, transpose_v(v), index, count, k_lens=k_lens, out=q if (recycle_q and out_dtype == BF16 and q.is_contiguous()) else None)
     return o.type(out_dtype)
 
 
