@@ -10,25 +10,6 @@
 namespace {
 
 typedef int mx_i8 __attribute__((ext_vector_type(8)));
-typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float mx_gelu_tanh(float x) {
-  const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;  // -2 sqrt(2/pi) log2(e)
-  const float t = __builtin_fmaf(x * x, 0.044715f, 1.0f);
-  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * t * c));
-}
-
-struct MxGemm {
-  const uint8_t *A, *As, *W, *Ws;   // rows of the output, columns of the output (transposed form: W, A)
-  int64_t M, N;
-  int K, kt;
-  const bf16_t* bias;
-  bf16_t* C;
-  int64_t ldc;
-  const bf16_t *R, *mod, *e;
-  int n_mod, gate_idx;
-  int64_t rows_per_batch;
-};
 
 // ---- the general kernel: any M and N, K % 32 == 0; 128 x 128 tiles, 4 waves of 64 x 64 -----------------------------------------------------
 template <int EPI>   // WAN_EPI_TRANSPOSED: the bias runs along the rows
@@ -118,6 +99,8 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_kernel(MxGemm p) {
 
 }  // namespace
 
+int wan_gemm_mxfp4m_try(const MxGemm& p, int epilogue, hipStream_t st);   // gemm_mxfp4m.hip
+
 extern "C" int64_t wan_gemm_mxfp4_scratch_bytes(int64_t M, int N, int K, int epilogue) { return 0; }
 
 extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C, int64_t ldc, int64_t M, int N, int K,
@@ -130,19 +113,21 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
   const bool tr = epilogue == WAN_EPI_TRANSPOSED;
   WAN_REQUIRE(ldc >= (tr ? M : N), "wan_gemm_mxfp4: ldc=%lld is smaller than a row of the output", (long long)ldc);
   MxGemm p = {tr ? W : A, tr ? w_scales : a_scales, tr ? A : W, tr ? a_scales : w_scales, tr ? N : M, tr ? M : N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx, rows_per_batch > 0 ? rows_per_batch : 1};
+  if (epilogue == WAN_EPI_GATE_RES) {
+    WAN_REQUIRE(R != nullptr, "wan_gemm_mxfp4: GATE_RES needs the residual R");
+    WAN_REQUIRE(gate_idx < 0 || (mod && e && gate_idx < n_mod && rows_per_batch > 0), "wan_gemm_mxfp4: bad gate args");
+  }
+  WAN_REQUIRE(epilogue >= WAN_EPI_NONE && epilogue <= WAN_EPI_TRANSPOSED, "wan_gemm_mxfp4: unknown epilogue %d", epilogue);
+  const int rc = wan_gemm_mxfp4m_try(p, epilogue, st);
+  if (rc >= 0) return rc;
   const int64_t tiles = ((p.M + 127) / 128) * ((p.N + 127) / 128);
   WAN_REQUIRE(tiles < ((int64_t)1 << 31), "wan_gemm_mxfp4: grid too large");
   const dim3 grid((unsigned)tiles), wg(256);
   switch (epilogue) {
     case WAN_EPI_NONE: hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_NONE>, grid, wg, 0, st, p); break;
     case WAN_EPI_GELU_TANH: hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_GELU_TANH>, grid, wg, 0, st, p); break;
-    case WAN_EPI_GATE_RES:
-      WAN_REQUIRE(R != nullptr, "wan_gemm_mxfp4: GATE_RES needs the residual R");
-      WAN_REQUIRE(gate_idx < 0 || (mod && e && gate_idx < n_mod && rows_per_batch > 0), "wan_gemm_mxfp4: bad gate args");
-      hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_GATE_RES>, grid, wg, 0, st, p);
-      break;
-    case WAN_EPI_TRANSPOSED: hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_TRANSPOSED>, grid, wg, 0, st, p); break;
-    default: WAN_REQUIRE(false, "wan_gemm_mxfp4: unknown epilogue %d", epilogue);
+    case WAN_EPI_GATE_RES: hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_GATE_RES>, grid, wg, 0, st, p); break;
+    default: hipLaunchKernelGGL(gemm_mxfp4_kernel<WAN_EPI_TRANSPOSED>, grid, wg, 0, st, p); break;
   }
   WAN_LAUNCH_CHECK();
   return 0;

@@ -4,6 +4,8 @@
 
 namespace {
 
+typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
+
 // where the scale byte of (row, block j of the row) lies; kt = tiles of 8 blocks along K
 __device__ __forceinline__ int64_t mxfp4_scale_at(int64_t row, int j, int kt) {
   const int r = (int)(row & 127);
@@ -40,4 +42,23 @@ __device__ __forceinline__ float mxfp4_value(uint32_t code) {
   return (code & 8u) ? -a : a;
 }
 
+__device__ __forceinline__ float mx_gelu_tanh(float x) {
+  const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;  // -2 sqrt(2/pi) log2(e)
+  const float t = __builtin_fmaf(x * x, 0.044715f, 1.0f);
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * t * c));
+}
+
 }  // namespace
+
+// a product's operands as the kernels see them: Y = the rows of the output, X = its columns (the transposed form: weights, tokens)
+struct MxGemm {
+  const uint8_t *A, *As, *W, *Ws;
+  int64_t M, N;
+  int K, kt;
+  const bf16_t* bias;
+  bf16_t* C;
+  int64_t ldc;
+  const bf16_t *R, *mod, *e;
+  int n_mod, gate_idx;
+  int64_t rows_per_batch;
+};
