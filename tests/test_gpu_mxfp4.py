@@ -138,7 +138,7 @@ def close(got, ref, err):
 
 
 SHAPES = [(1, 8, 32), (1, 5120, 512), (2, 64, 64), (5, 200, 96), (16, 256, 256), (33, 1000, 320), (128, 128, 256), (130, 264, 544), (257, 513, 768), (300, 1536, 1536), (1000, 640, 2080),
-          (1024, 2048, 512), (4097, 4096, 768), (20000, 1024, 1280), (1, 30720, 5120), (64, 5120, 13824)]
+          (1024, 2048, 512), (4097, 4096, 768), (20000, 1024, 1280), (9001, 1160, 1056), (40000, 264, 32), (5000, 2056, 2848), (1, 30720, 5120), (64, 5120, 13824)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -173,6 +173,21 @@ def test_linear_every_epilogue(ops, M, N, K):
     vt = ops.linear_mxfp4(x, *wm, bias, epilogue=3)
     assert vt.shape == (N, (M + 63) // 64 * 64) and (vt[:, M:] == 0).all()
     close(vt[:, :M], y.t(), (err + 2.0 ** -8 * (y.abs() + err)).t())
+
+
+def test_gate_rows_of_many_batches(ops):
+    """Batches shorter than a tile, and of a tile's size and a little more: every row takes its own batch's gate."""
+    g = gen(9)
+    for nb, rpb, N, K in ((50, 100, 2048, 256), (19, 257, 2304, 320), (1, 5000, 2304, 256)):
+        M = nb * rpb
+        x, xm, wm, xd, wd = operands(ops, g, M, N, K)
+        y, err = linear_ref(xd, wd, None)
+        r = torch.randn(M, N, generator=g, device="cuda").to(BF)
+        mod, e = torch.randn(6, N, generator=g, device="cuda").to(BF), torch.randn(nb, 6, N, generator=g, device="cuda").to(BF)
+        gate = (mod[2].to(F64) + e[:, 2].to(F64)).repeat_interleave(rpb, 0)
+        out = r.to(F64) + y * gate
+        bound = err * gate.abs() + 2.0 ** -22 * (r.to(F64).abs() + (y * gate).abs())
+        close(ops.linear_mxfp4(None, *wm, epilogue=2, residual=r, mod=mod, e=e, gate_idx=2, x_mx=xm), out, bound + 2.0 ** -8 * (out.abs() + bound))
 
 
 def test_linear_leaves_what_lies_past_the_result(ops):

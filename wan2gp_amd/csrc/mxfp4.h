@@ -6,12 +6,6 @@ namespace {
 
 typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
 
-// where the scale byte of (row, block j of the row) lies; kt = tiles of 8 blocks along K
-__device__ __forceinline__ int64_t mxfp4_scale_at(int64_t row, int j, int kt) {
-  const int r = (int)(row & 127);
-  return ((row >> 7) * kt + (j >> 3)) * 1024 + (j & 3) * 256 + (r >> 3) * 16 + ((j >> 2) & 1) * 8 + (r & 7);
-}
-
 // the e8m0 byte of a block whose largest magnitude has the float bits `amax`
 __device__ __forceinline__ uint32_t mxfp4_scale(uint32_t amax) {
   if (amax >= 0x7f800000u) return 255u;
@@ -19,27 +13,29 @@ __device__ __forceinline__ uint32_t mxfp4_scale(uint32_t amax) {
   return (uint32_t)min(max(e, 0), 252);
 }
 
-__device__ __forceinline__ uint32_t mxfp4_code(float y) {
-  const float a = fabsf(y);
-  const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-  return c | (__float_as_uint(y) >> 31 << 3);
+// eight values of a block with scale byte e8 -> their codes, the first in the lowest nibble.  v_cvt_scalef32_pk_fp4_f32 rounds to nearest even and
+// stops at 6 (checked for every bf16 value); the scale is applied by v_ldexp in front of it, which is exact over the whole exponent range.
+__device__ __forceinline__ uint32_t mxfp4_encode8(const float* f, uint32_t e8) {
+  if (e8 == 255u) return 0u;
+  const int sh = 127 - (int)e8;
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, ldexpf(f[0], sh), ldexpf(f[1], sh), 1.0f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, ldexpf(f[2], sh), ldexpf(f[3], sh), 1.0f, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, ldexpf(f[4], sh), ldexpf(f[5], sh), 1.0f, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, ldexpf(f[6], sh), ldexpf(f[7], sh), 1.0f, 3);
+  return c;
 }
-
-// eight values of a block -> their codes (lowest nibble first) and the block's scale byte
-__device__ __forceinline__ uint32_t mxfp4_encode8(const float* f, uint32_t amax, uint32_t& codes) {
-  const uint32_t e8 = mxfp4_scale(amax);
-  codes = 0;
-  if (e8 != 255u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) codes |= mxfp4_code(ldexpf(f[i], 127 - (int)e8)) << (4 * i);
+// the values they stand for
+__device__ __forceinline__ void mxfp4_decode8(uint32_t c, uint32_t e8, float* f) {
+  const int sh = (int)e8 - 127;
+#define MX_PAIR(B)                                                             \
+  {                                                                            \
+    const wan_f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, B);  \
+    f[2 * B] = e8 == 255u ? __uint_as_float(0x7fc00000u) : ldexpf(v[0], sh);   \
+    f[2 * B + 1] = e8 == 255u ? __uint_as_float(0x7fc00000u) : ldexpf(v[1], sh); \
   }
-  return e8;
-}
-
-__device__ __forceinline__ float mxfp4_value(uint32_t code) {
-  const uint32_t m = code & 7u;
-  const float a = m < 4u ? 0.5f * (float)m : (m == 4u ? 2.f : m == 5u ? 3.f : m == 6u ? 4.f : 6.f);
-  return (code & 8u) ? -a : a;
+  MX_PAIR(0) MX_PAIR(1) MX_PAIR(2) MX_PAIR(3)
+#undef MX_PAIR
 }
 
 __device__ __forceinline__ float mx_gelu_tanh(float x) {
