@@ -27,26 +27,6 @@ struct MxmFrags {
   mx_u4 y[8], x[8];
 };
 
-// D += A B over 128 values with both blocks' scales; T, U: the bytes of sy, sx
-template <int T, int U>
-__device__ __forceinline__ void mfma_mx(f32x4& acc, const mx_u4& ya, const mx_u4& xb, uint32_t sy, uint32_t sx) {
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
-               : "+a"(acc)
-               : "v"(ya), "v"(xb), "v"(sy), "v"(sx), "n"(T & 1), "n"(U & 1), "n"(T >> 1), "n"(U >> 1));
-}
-__device__ __forceinline__ void mxm_dma16(uint32_t voff, const mx_u4& rsrc, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds_addr) : "memory");
-}
-__device__ __forceinline__ mx_u4 mxm_rsrc(const char* base, uint32_t bytes) {
-  const uint64_t b = (uint64_t)base;
-  mx_u4 r;
-  r[0] = (uint32_t)b;
-  r[1] = (uint32_t)(b >> 32) & 0xffffu;  // stride 0
-  r[2] = bytes;                          // beyond: zeros
-  r[3] = 0x00020000u;
-  return r;
-}
-
 // MFMA m of a k-step: y tile m >> 3, x tile m & 7
 template <int KS, int M0, int M1, class F>
 __device__ __forceinline__ void mxm_run(f32x4 (&acc)[8][8], const MxmFrags& f, const mx_u4& sy, const mx_u4& sx, F&& gap) {
@@ -98,8 +78,8 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   const uint32_t smem_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   const int nk = p.kt;
   int ky = 0, kx = 0;  // the stages the two streams point at; they stop at the last one
-  auto y_piece = [&](int slot, int i) { mxm_dma16(yofs[i], mxm_rsrc(ybase, yrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
-  auto x_piece = [&](int slot, int i) { mxm_dma16(xofs[i], mxm_rsrc(xbase, xrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
+  auto y_piece = [&](int slot, int i) { mx_dma16(yofs[i], mx_rsrc(ybase, yrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
+  auto x_piece = [&](int slot, int i) { mx_dma16(xofs[i], mx_rsrc(xbase, xrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
   auto y_advance = [&]() { const int s = ky + 1 < nk ? MXM_ROW : 0; ybase += s; yrec -= s; ky += s ? 1 : 0; };
   auto x_advance = [&]() { const int s = kx + 1 < nk ? MXM_ROW : 0; xbase += s; xrec -= s; kx += s ? 1 : 0; };
 
@@ -292,7 +272,7 @@ int wan_gemm_mxfp4m_try(const MxGemm& p, int epilogue, hipStream_t st) {
   if (epilogue == WAN_EPI_GATE_RES && p.gate_idx >= 0 && p.rows_per_batch < MXM_BM) return -1;
   if (256 * (int64_t)(p.K / 2) + 256 >= ((int64_t)1 << 31) || 256 * p.ldc * 2 + 512 >= ((int64_t)1 << 31)) return -1;   // 32-bit offsets inside a tile
   const int64_t ty = (p.M + MXM_BM - 1) / MXM_BM, tx = (p.N + MXM_BN - 1) / MXM_BN;
-  if (ty * tx < 160 || ty * tx >= ((int64_t)1 << 31)) return -1;
+  if (ty * tx >= ((int64_t)1 << 31)) return -1;
   const dim3 grid((unsigned)(ty * tx)), wg(256);
   const int group = epilogue == WAN_EPI_TRANSPOSED ? 8 : 4;
   switch (epilogue) {

@@ -38,6 +38,28 @@ __device__ __forceinline__ void mxfp4_decode8(uint32_t c, uint32_t e8, float* f)
 #undef MX_PAIR
 }
 
+// D += A B over 128 values with both blocks' scales; T, U: the bytes of sy, sx.  Accumulators pinned to the accumulator file (builtin MFMAs had them copied
+// back and forth: 92 register moves a stage of 32 MFMAs)
+template <int T, int U>
+__device__ __forceinline__ void mfma_mx(f32x4& acc, const mx_u4& ya, const mx_u4& xb, uint32_t sy, uint32_t sx) {
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%6,0] op_sel_hi:[%7,%8,0] cbsz:4 blgp:4"
+               : "+a"(acc)
+               : "v"(ya), "v"(xb), "v"(sy), "v"(sx), "n"(T & 1), "n"(U & 1), "n"(T >> 1), "n"(U >> 1));
+}
+// One LDS-DMA piece (16 bytes a lane, 1 KB a wave) as inline asm: hipcc's waitcnt pass does not see it, completion is counted by hand
+__device__ __forceinline__ void mx_dma16(uint32_t voff, const mx_u4& rsrc, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds_addr) : "memory");
+}
+__device__ __forceinline__ mx_u4 mx_rsrc(const char* base, uint32_t bytes) {
+  const uint64_t b = (uint64_t)base;
+  mx_u4 r;
+  r[0] = (uint32_t)b;
+  r[1] = (uint32_t)(b >> 32) & 0xffffu;  // stride 0
+  r[2] = bytes;                          // beyond: zeros
+  r[3] = 0x00020000u;
+  return r;
+}
+
 __device__ __forceinline__ float mx_gelu_tanh(float x) {
   const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;  // -2 sqrt(2/pi) log2(e)
   const float t = __builtin_fmaf(x * x, 0.044715f, 1.0f);

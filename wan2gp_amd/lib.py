@@ -99,9 +99,12 @@ SIGNATURES = {
     "wan_mxfp4_scale_bytes": (c_int64, [c_int64, c_int64]),
     "wan_mxfp4_quantize": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "wan_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),
-    "wan_gemm_mxfp4_scratch_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "wan_gemm_mxfp4_scratch_bytes": (c_int64, [c_int64, c_int, c_int]),
     "wan_gemm_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
                                c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_int64, c_void_p]),
+    "wan_linear_mxfp4_scratch_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "wan_linear_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p,
+                                 c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_int64, c_void_p]),
     "wan_block_mean": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p]),
     "wan_select_blocks_scratch_bytes": (c_int64, [c_int, c_int, c_int64, c_int64]),
     "wan_select_blocks": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int,

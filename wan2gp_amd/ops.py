@@ -329,6 +329,23 @@ def _same_device(first, *others):
             raise _L.WanHipError(f"all tensors must be on one device, got {first.device} and {t.device}")
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(device, fn, *args):
+    """fn(*args, the current stream of `device`) with `device` current, whichever is outside.  (The stream is asked for by its handle: the object that
+    torch.cuda.current_stream() makes costs as much as the launch of a small kernel, 3 us.)"""
+    i = device.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != 0:
+        check(rc, fn.__name__)
+
+
 def _token_strides(t, name):
     """(row, batch) strides in elements of a bf16 [B, L, H, 128] tensor whose heads lie side by side in a row: a slice of a fused projection
     is taken as it is."""
@@ -365,8 +382,7 @@ def block_mean(x, block, lens=None):
         raise _L.WanHipError("block must be positive")
     out = torch.empty(B, H, (L + block - 1) // block, 128, dtype=torch.float32, device=x.device)
     if out.numel():
-        with torch.cuda.device(x.device):
-            check(_L.load().wan_block_mean(ptr(x), row, batch, ptr(lens), ptr(out), B, L, H, block, stream_ptr()), "wan_block_mean")
+        _call(x.device, _L.load().wan_block_mean, x.data_ptr(), row, batch, _addr(lens), out.data_ptr(), B, L, H, block)
     return out
 
 
@@ -389,10 +405,8 @@ def select_blocks(q_mean, k_mean, keep, k_lens=None):
         return index, count
     lib = _L.load()
     need = int(lib.wan_select_blocks_scratch_bytes(B, H, nq, nk))
-    with torch.cuda.device(q_mean.device):
-        ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device)
-        check(lib.wan_select_blocks(ptr(q_mean), ptr(k_mean), ptr(k_lens), ptr(index), ptr(count), B, Bk, H, Hk, nq, nk, keep, ptr(ws), need, stream_ptr()),
-              "wan_select_blocks")
+    ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device)
+    _call(q_mean.device, lib.wan_select_blocks, q_mean.data_ptr(), k_mean.data_ptr(), _addr(k_lens), index.data_ptr(), count.data_ptr(), B, Bk, H, Hk, nq, nk, keep, ws.data_ptr(), need)
     return index, count
 
 
@@ -425,16 +439,14 @@ def sparse_attention(q, k, vt, block_index, block_count=None, k_lens=None, out=N
         return out.zero_()
     lib = _L.load()
     need = int(lib.wan_sparse_attention_scratch_bytes(B, Lq, H, keep))
-    with torch.cuda.device(q.device):
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        check(lib.wan_sparse_attention(ptr(q), q_row, q_batch, ptr(k), k_row, k_batch, ptr(vt), ptr(out), ptr(block_index), ptr(block_count), ptr(k_lens), B, Bk, Lq, Lk,
-                                       ldv, H, Hk, keep, 1 if q_prescaled else 0, ptr(ws), need, stream_ptr()), "wan_sparse_attention")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _call(q.device, lib.wan_sparse_attention, q.data_ptr(), q_row, q_batch, k.data_ptr(), k_row, k_batch, vt.data_ptr(), out.data_ptr(), block_index.data_ptr(), _addr(block_count), _addr(k_lens),
+          B, Bk, Lq, Lk, ldv, H, Hk, keep, 1 if q_prescaled else 0, _addr(ws), need)
     return out
 
 
-def mxfp4_quantize(x):
-    """x [..., K] bf16 (rows of a 2-D tensor may be strided) -> (codes uint8 [..., K/2], scales uint8): 4-bit floating point with a power of two per
-    32 values; the layouts are those of include/wanhip.h (the scales in the order of the matrix instruction's lanes)."""
+def _mx_rows(x):
+    """(M, K, row stride) of a bf16 tensor that is to be quantised along its last dimension"""
     if not x.is_cuda:
         raise _L.WanHipError("x must be a CUDA(HIP) tensor -- libwanhip has no CPU path")
     if x.dtype != BF16:
@@ -442,19 +454,22 @@ def mxfp4_quantize(x):
     if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
         raise _L.WanHipError(f"the last dimension of x must be a positive multiple of 32, got {list(x.shape)}")
     K = x.shape[-1]
-    M = x.numel() // K
     if x.is_contiguous():
-        row = K
-    elif x.dim() == 2 and x.stride(1) == 1:
-        row = x.stride(0)
-    else:
-        raise _L.WanHipError("x must be contiguous, or 2-D with contiguous rows")
+        return x.numel() // K, K, K
+    if x.dim() == 2 and x.stride(1) == 1:
+        return x.shape[0], K, (x.stride(0) if x.shape[0] > 1 else K)
+    raise _L.WanHipError("x must be contiguous, or 2-D with contiguous rows")
+
+
+def mxfp4_quantize(x):
+    """x [..., K] bf16 (rows of a 2-D tensor may be strided) -> (codes uint8 [..., K/2], scales uint8): 4-bit floating point with a power of two per
+    32 values; the layouts are those of include/wanhip.h (the scales in the order of the matrix instruction's lanes)."""
+    M, K, row = _mx_rows(x)
     lib = _L.load()
     codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(int(lib.wan_mxfp4_scale_bytes(M, K)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(lib.wan_mxfp4_scale_bytes(M, K), dtype=torch.uint8, device=x.device)
     if M:
-        with torch.cuda.device(x.device):
-            check(lib.wan_mxfp4_quantize(ptr(x), row, ptr(codes), ptr(scales), M, K, stream_ptr()), "wan_mxfp4_quantize")
+        _call(x.device, lib.wan_mxfp4_quantize, x.data_ptr(), row, codes.data_ptr(), scales.data_ptr(), M, K)
     return codes, scales
 
 
@@ -465,7 +480,7 @@ def _mx_operand(codes, scales, name):
     _same_device(codes, scales)
     K = codes.shape[-1] * 2
     M = codes.numel() // (K // 2)
-    need = int(_L.load().wan_mxfp4_scale_bytes(M, K))
+    need = _L.load().wan_mxfp4_scale_bytes(M, K)
     if scales.numel() != need:
         raise _L.WanHipError(f"{name} scales must hold {need} bytes, got {scales.numel()}")
     return M, K
@@ -476,8 +491,7 @@ def mxfp4_dequantize(codes, scales):
     M, K = _mx_operand(codes, scales, "codes")
     out = torch.empty(*codes.shape[:-1], K, dtype=BF16, device=codes.device)
     if M:
-        with torch.cuda.device(codes.device):
-            check(_L.load().wan_mxfp4_dequantize(ptr(codes), ptr(scales), ptr(out), M, K, stream_ptr()), "wan_mxfp4_dequantize")
+        _call(codes.device, _L.load().wan_mxfp4_dequantize, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, K)
     return out
 
 
@@ -491,34 +505,34 @@ def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, r
         raise _L.WanHipError(f"weight_codes must be [N, K / 2], got {list(weight_codes.shape)}")
     N, K = _mx_operand(weight_codes, weight_scales, "weight_codes")
     if x_mx is None:
-        if x.shape[-1] != K:
-            raise _L.WanHipError(f"x has rows of {x.shape[-1]} values, the weight of {K}")
-        x_mx = mxfp4_quantize(x)
-    xc, xs = x_mx
-    M, Kx = _mx_operand(xc, xs, "x_mx")
+        M, Kx, row = _mx_rows(x)
+        shape = x.shape[:-1]
+    else:
+        M, Kx = _mx_operand(*x_mx, "x_mx")
+        shape = x_mx[0].shape[:-1]
     if Kx != K:
         raise _L.WanHipError(f"x has rows of {Kx} values, the weight of {K}")
-    _same_device(xc, weight_codes, bias, residual, mod, e, out)
+    _same_device(weight_codes, x if x_mx is None else x_mx[0], bias, residual, mod, e, out)
     if bias is not None and bias.numel() != N:
         raise _L.WanHipError(f"bias must hold {N} values")
     if epilogue == EPI_TRANSPOSED:
         ldc = ldc or ((M + 63) // 64) * 64
         if out is None:
-            out = torch.zeros(N, ldc, dtype=BF16, device=xc.device)
-        shape_ok = out.numel() >= N * ldc and ldc >= M
+            out = torch.zeros(N, ldc, dtype=BF16, device=weight_codes.device)
+        if out.numel() < N * ldc or ldc < M:
+            raise _L.WanHipError(f"out {list(out.shape)} does not hold the result ({N} x {M}, ldc {ldc})")
     else:
         ldc = N
         if out is None:
-            out = torch.empty(*xc.shape[:-1], N, dtype=BF16, device=xc.device)
-        shape_ok = out.numel() == M * N
-    if not shape_ok:
-        raise _L.WanHipError(f"out {list(out.shape)} does not hold the result ({M} x {N}, ldc {ldc})")
+            out = torch.empty(*shape, N, dtype=BF16, device=weight_codes.device)
+        if out.numel() != M * N:
+            raise _L.WanHipError(f"out {list(out.shape)} does not hold the result ({M} x {N})")
     n_mod, nb = 0, 1
     if epilogue == EPI_GATE_RES:
         if residual is None or residual.numel() != M * N:
             raise _L.WanHipError(f"the gated residual needs a residual of {M} x {N} values")
         if gate_idx >= 0:
-            if mod is None or e is None or mod.numel() % N or gate_idx >= mod.numel() // N or e.numel() == 0 or e.numel() % mod.numel():
+            if mod is None or e is None or mod.numel() == 0 or mod.numel() % N or gate_idx >= mod.numel() // N or e.numel() == 0 or e.numel() % mod.numel():
                 raise _L.WanHipError("the gate needs mod [.., n_mod, N] with row gate_idx, and e [batches, n_mod, N]")
             n_mod = mod.numel() // N
             nb = e.numel() // mod.numel()
@@ -527,11 +541,14 @@ def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, r
     if M == 0:
         return out
     lib = _L.load()
-    need = int(lib.wan_gemm_mxfp4_scratch_bytes(M, N, K, epilogue))
-    with torch.cuda.device(xc.device):
-        ws = torch.empty(need, dtype=torch.uint8, device=xc.device) if need else None
-        check(lib.wan_gemm_mxfp4(ptr(xc), ptr(xs), ptr(weight_codes), ptr(weight_scales), ptr(bias), ptr(out), ldc, M, N, K, epilogue, ptr(residual), ptr(mod), ptr(e),
-                                 n_mod, gate_idx, M // nb, ptr(ws), need, stream_ptr()), "wan_gemm_mxfp4")
+    need = (lib.wan_linear_mxfp4_scratch_bytes if x_mx is None else lib.wan_gemm_mxfp4_scratch_bytes)(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=weight_codes.device) if need else None
+    tail = (weight_codes.data_ptr(), weight_scales.data_ptr(), _addr(bias), out.data_ptr(), ldc, M, N, K, epilogue, _addr(residual), _addr(mod), _addr(e), n_mod, gate_idx,
+            M // nb, _addr(ws), need)
+    if x_mx is None:
+        _call(weight_codes.device, lib.wan_linear_mxfp4, x.data_ptr(), row, *tail)
+    else:
+        _call(weight_codes.device, lib.wan_gemm_mxfp4, x_mx[0].data_ptr(), x_mx[1].data_ptr(), *tail)
     return out
 
 
