@@ -12,6 +12,7 @@
 namespace {
 
 constexpr int Q_BLOCK = 128;
+constexpr float LAZY = 32.f;   // how far above its reference (log2) a row's scores may lie
 constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 
 struct SparseArgs {
@@ -20,7 +21,7 @@ struct SparseArgs {
   int64_t q_row, q_batch, k_row, k_batch, ldv, Lq, Lk;
   const int *index, *count, *k_lens;
   int B, Bk, H, Hk, nq, keep;
-  float scale_log2e;
+  int q_prescaled;
 };
 
 __device__ __forceinline__ f32x4 mfma16(const mfma_bf16x8& a, const mfma_bf16x8& b, const f32x4& c) {
@@ -79,13 +80,32 @@ __global__ __launch_bounds__(256, 2) void attn_sparse_kernel(SparseArgs p) {
     const int64_t r = min(q0 + 16 * qt + n, p.Lq - 1);
     const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) qf[qt][ks] = *reinterpret_cast<const mfma_bf16x8*>(qp + 32 * ks);
+    for (int ks = 0; ks < 4; ++ks) {
+      uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
+      if (!p.q_prescaled) {   // the scale folded into q and rounded with it (as the dense kernels do): no multiplication per score
+        float f[8];
+        unpack8(w, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
+        w = pack8(f);
+      }
+      qf[qt][ks] = __builtin_bit_cast(mfma_bf16x8, w);
+    }
   }
-  f32x4 acc[8][2] = {};
-  float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const uint4 one_bits = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  const mfma_bf16x8 ones = __builtin_bit_cast(mfma_bf16x8, one_bits);
+  f32x4 acc[8][2], l[2], negm[2];
+#pragma unroll
+  for (int qt = 0; qt < 2; ++qt) {
+    l[qt] = negm[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) acc[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  bool unset[2] = {true, true};   // the row has no reference yet
 
   int e = next(0), st = 0;
   if (e < entries) fetch(list[e], 0);
+  bool force = true;
   while (e < entries) {
     const int blk = __builtin_amdgcn_readfirstlane(list[e]);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -101,52 +121,74 @@ __global__ __launch_bounds__(256, 2) void attn_sparse_kernel(SparseArgs p) {
       }
       __syncthreads();
     }
+    // S - m: the reference enters as the C operand of each tile's first product
     f32x4 s[4][2];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      s[kt][0] = s[kt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const mfma_bf16x8 kf = *(lds_frag*)(lds + st * IMG + (16 * kt + n) * 256 + (((4 * ks + g) ^ n) << 4));
-        s[kt][0] = mfma16(kf, qf[0][ks], s[kt][0]);
-        s[kt][1] = mfma16(kf, qf[1][ks], s[kt][1]);
+        s[kt][0] = mfma16(kf, qf[0][ks], ks == 0 ? negm[0] : s[kt][0]);
+        s[kt][1] = mfma16(kf, qf[1][ks], ks == 0 ? negm[1] : s[kt][1]);
       }
+    if (rem < KVBLK) {
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + i >= rem) s[kt][qt][i] = -INFINITY;
+    }
+    float top[2];
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      top[qt] = fmaxf(s[0][qt][0], s[0][qt][1]);
+#pragma unroll
+      for (int k = 2; k < 16; k += 2) top[qt] = fmaxf(top[qt], fmaxf(s[k >> 2][qt][k & 3], s[(k + 1) >> 2][qt][(k + 1) & 3]));
+    }
+    // The reference m of a row follows its maximum only when a score lies more than 2^LAZY above it: until then the weights 2^(s - m) are merely
+    // large numbers, which bf16 and fp32 carry with the same relative precision.  The first block sets it.
+    if (force || __any(fmaxf(top[0], top[1]) > LAZY)) {
+      bool open = false;
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt) {
+        float t = top[qt];
+        t = fmaxf(t, __shfl_xor(t, 16, 64));
+        t = fmaxf(t, __shfl_xor(t, 32, 64));
+        const bool none = t == -INFINITY;      // (every product so far is -inf: the row waits for a block with another)
+        if (none || (!unset[qt] && t <= LAZY)) t = 0.f;
+        unset[qt] = unset[qt] && none;
+        open |= unset[qt];
+        const float a = __builtin_amdgcn_exp2f(-t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { negm[qt][i] -= t; l[qt][i] *= a; }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) acc[dt][qt] *= a;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kt][qt][i] -= t;
+      }
+      force = __any(open);
     }
     mfma_bf16x8 pf[2][2];
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) {
-      float top = -INFINITY;
+    for (int qt = 0; qt < 2; ++qt)
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[kt][qt][i] * p.scale_log2e;
-          if (rem < KVBLK && 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + i >= rem) x = -INFINITY;
-          s[kt][qt][i] = x;
-          top = fmaxf(top, x);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(mx[qt], top), ref = mn == -INFINITY ? 0.f : mn;
-      const float a = __builtin_amdgcn_exp2f(mx[qt] - ref);
-      mx[qt] = mn;
-      l[qt] *= a;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) acc[dt][qt] *= a;
-      uint32_t w[8];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = __builtin_amdgcn_exp2f(s[kt][qt][i] - ref);
-          l[qt] += x[i];
-        }
-        w[2 * kt] = cvt_pk(x[0], x[1]);
-        w[2 * kt + 1] = cvt_pk(x[2], x[3]);
+      for (int c = 0; c < 2; ++c) {
+        uint4 w;
+        w.x = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c][qt][0]), __builtin_amdgcn_exp2f(s[2 * c][qt][1]));
+        w.y = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c][qt][2]), __builtin_amdgcn_exp2f(s[2 * c][qt][3]));
+        w.z = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c + 1][qt][0]), __builtin_amdgcn_exp2f(s[2 * c + 1][qt][1]));
+        w.w = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c + 1][qt][2]), __builtin_amdgcn_exp2f(s[2 * c + 1][qt][3]));
+        pf[qt][c] = __builtin_bit_cast(mfma_bf16x8, w);
       }
-      pf[qt][0] = __builtin_bit_cast(mfma_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-      pf[qt][1] = __builtin_bit_cast(mfma_bf16x8, make_uint4(w[4], w[5], w[6], w[7]));
+    // the row sums are one more tile of the product, over a V of ones: of the rounded weights, as the numerator's, and already over all lanes
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[0] = mfma16(ones, pf[0][c], l[0]);
+      l[1] = mfma16(ones, pf[1][c], l[1]);
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
@@ -161,9 +203,7 @@ __global__ __launch_bounds__(256, 2) void attn_sparse_kernel(SparseArgs p) {
   }
 #pragma unroll
   for (int qt = 0; qt < 2; ++qt) {
-    float t = l[qt];
-    t += __shfl_xor(t, 16, 64);
-    t += __shfl_xor(t, 32, 64);
+    const float t = l[qt][0];
     const float inv = t == 0.f ? 0.f : 1.f / t;   // a row without keys: zeros
     const int64_t r = q0 + 16 * qt + n;
     if (r < p.Lq) {
@@ -200,7 +240,7 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   WAN_REQUIRE(k_row < ((int64_t)1 << 24) && ldv < ((int64_t)1 << 23), "wan_sparse_attention: a row of k of %lld elements or %lld keys exceed the kernel's offsets", (long long)k_row, (long long)ldv);
   const int64_t nq = (Lq + Q_BLOCK - 1) / Q_BLOCK;
   WAN_REQUIRE(nq * H * B < ((int64_t)1 << 31), "wan_sparse_attention: grid too large");
-  SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled ? 1.f : SPARSE_SCALE_LOG2E};
+  SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled};
   hipLaunchKernelGGL(attn_sparse_kernel, dim3((unsigned)(nq * H * B)), dim3(256), 0, as_stream(stream), a);
   WAN_LAUNCH_CHECK();
   return 0;
