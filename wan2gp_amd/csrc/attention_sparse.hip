@@ -15,6 +15,261 @@ constexpr int Q_BLOCK = 128;
 constexpr float LAZY = 32.f;   // how far above its reference (log2) a row's scores may lie
 constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 
+// ---- 2 waves x 64 queries ----------------------------------------------------------------------------------------------------------------------
+// One wave per SIMD with the whole register file, its instruction stream laid out by hand as attention_w16n.hip's: 128 MFMAs of 16 cycles a tile
+// (A 0 .. 31: S_a, B 32 .. 63: PV_b of the tile before, C 64 .. 95: S_b, D 96 .. 127: PV_a; a, b: the wave's q tiles 0, 1 and 2, 3), one gap of up
+// to four issue slots behind each.  What is different here:
+//   * two waves to a list, so that a block of 128 queries has a list of its own, and two such workgroups to a CU: 80 KB of LDS each, K in a ring of
+//     two images and V^T in one of three (K(t) is in registers by the time K(t + 2) is fetched, V^T(t) is read in the middle of tile t);
+//   * the tiles' addresses come from the list, one scalar load a tile ahead of its use;
+//   * the softmax needs no bound on the scores: a half's maximum is taken (v_max3) between its last S tile and its first exp2, and only a score 2^LAZY
+//     above the row's reference, the first tile and tiles that end inside leave the straight path (cold16);
+//   * row sums by v_dot2_f32_bf16 over the packed pairs: one instruction for two scores, and of the rounded weights, as the product's.
+// Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 44 + 2 k, of b's behind 108 + 2 k, running into the next tile (k = 10 behind its
+// MFMA 0); a pair is packed in the odd gap behind its second exp2 and summed one odd gap later; maxima of a in the odd gaps 29 .. 43, of b 93 .. 107; DMA of tile
+// t + 2 in the odd gaps 3 .. 33; V^T(t) fragments 41 .. 71, K(t + 1) fragments 67 .. 97.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct SHalf {
+  f32x4 accO[8][2];   // O^T tiles [d tile][q tile]
+  f32x4 s[4][2];      // S^T - m [kv tile][q tile]
+  u32x4 pk[4];        // P^T fragments, f = 2 c + q tile
+  float p0, p1;       // the exp2 pair whose pack is pending
+  float l[2], top[2]; // this lane's share of the row sums; maxima of the current tile
+};
+__device__ __forceinline__ void sp_qk0(f32x4& d, const mfma_bf16x8& k, const mfma_bf16x8& q, const f32x4& c) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %3" : "=&v"(d) : "v"(k), "a"(q), "v"(c));
+}
+__device__ __forceinline__ void sp_qk(f32x4& d, const mfma_bf16x8& k, const mfma_bf16x8& q) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(k), "a"(q));
+}
+__device__ __forceinline__ void sp_pv(f32x4& acc, const mfma_bf16x8& v, const mfma_bf16x8& p) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "a"(v), "v"(p));
+}
+// MFMA i = 0 .. 31 of an S phase: k-step i >> 3, kv tile (i >> 1) & 3, q tile i & 1; of a PV phase: fragment f = i >> 3, d tile i & 7
+__device__ __forceinline__ void sp_s_step(SHalf& x, const mfma_bf16x8 (&kf)[4][4], const mfma_bf16x8 (&qf)[4][4], const f32x4 (&negm)[4], int qt0, int i) {
+  const int ks = i >> 3, kt = (i >> 1) & 3, qt = i & 1;
+  if (ks == 0) sp_qk0(x.s[kt][qt], kf[kt][0], qf[qt0 + qt][0], negm[qt0 + qt]);
+  else sp_qk(x.s[kt][qt], kf[kt][ks], qf[qt0 + qt][ks]);
+}
+__device__ __forceinline__ void sp_pv_step(SHalf& x, const mfma_bf16x8 (&vf)[8][2], int i) {
+  const int f = i >> 3, dt = i & 7;
+  sp_pv(x.accO[dt][f & 1], vf[dt][f >> 1], __builtin_bit_cast(mfma_bf16x8, x.pk[f]));
+}
+// score k = 0 .. 31 of a half in the order its fragments are needed: f = k >> 3, then kv tile parity, then register
+__device__ __forceinline__ float sp_score(const SHalf& x, int k) {
+  const int f = k >> 3;
+  return x.s[2 * (f >> 1) + ((k >> 2) & 1)][f & 1][k & 3];
+}
+__device__ __forceinline__ void sp_exp(SHalf& x, int k) {
+  // (asm: behind the builtin hipcc puts an s_nop in front of the pack, not counting the MFMA that stands between as the wait state it is)
+  if (k & 1) asm volatile("v_exp_f32 %0, %1" : "=v"(x.p1) : "v"(sp_score(x, k)));
+  else asm volatile("v_exp_f32 %0, %1" : "=v"(x.p0) : "v"(sp_score(x, k)));
+}
+__device__ __forceinline__ void sp_pack(SHalf& x, int k) {   // behind the odd score k
+  const int j = k >> 1;
+  x.pk[j >> 2][j & 3] = cvt_pk(x.p0, x.p1);
+  asm volatile("" : "+v"(x.pk[j >> 2]));
+}
+__device__ __forceinline__ void sp_sum(SHalf& x, int k) {    // the pair that ends with the odd score k
+  const int j = k >> 1, qt = (k >> 3) & 1;
+  const uint32_t pair = x.pk[j >> 2][j & 3];   // (a value of its own: bit_cast of a vector's element takes element 0)
+  x.l[qt] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, pair), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), x.l[qt], false);
+  asm volatile("" : "+v"(x.l[qt]));
+}
+// step j = 0 .. 7 of the maximum over a q tile's 16 scores, in the order the S tiles are finished
+template <int J>
+__device__ __forceinline__ void sp_max(SHalf& x, int qt) {
+  // (asm: fmaxf of values that hipcc has not seen computed comes with a v_max x, x in front)
+  if constexpr (J == 0) asm volatile("v_max3_f32 %0, %1, %2, %3" : "=v"(x.top[qt]) : "v"(x.s[0][qt][0]), "v"(x.s[0][qt][1]), "v"(x.s[0][qt][2]));
+  else if constexpr (J < 7) {
+    constexpr int A = 2 * J + 1, B = 2 * J + 2;
+    asm volatile("v_max3_f32 %0, %0, %1, %2" : "+v"(x.top[qt]) : "v"(x.s[A >> 2][qt][A & 3]), "v"(x.s[B >> 2][qt][B & 3]));
+  } else asm volatile("v_max_f32 %0, %0, %1" : "+v"(x.top[qt]) : "v"(x.s[3][qt][3]));
+}
+// The lane's number, opaque: what the rare paths and the epilogue derive from it is not computed ahead of the tile loop and kept in registers
+__device__ __forceinline__ uint32_t sp_lane() {
+  uint32_t lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+// What leaves the straight path: the scores of a tile's keys past the end become -inf, and a row's reference moves to its maximum -- for the first
+// time (the row sum is 0: until a key has a finite score the reference is 0 and waits), or because a score lies more than 2^LAZY above it.
+// Returns whether a row still waits.
+__device__ __forceinline__ bool sp_cold(SHalf& x, f32x4* negm, int rem) {
+  bool open = false;
+  const int lim = rem - 8 * (int)(sp_lane() >> 4);
+#pragma unroll
+  for (int qt = 0; qt < 2; ++qt) {
+    float t = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x.s[kt][qt][i] = 32 * (kt >> 1) + 4 * (kt & 1) + i >= lim ? -INFINITY : x.s[kt][qt][i];
+        asm volatile("" : "+v"(x.s[kt][qt][i]));
+        t = fmaxf(t, x.s[kt][qt][i]);
+      }
+    t = fmaxf(t, __shfl_xor(t, 16, 64));
+    t = fmaxf(t, __shfl_xor(t, 32, 64));
+    float l = x.l[qt];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const bool first = l == 0.f, none = t == -INFINITY;
+    open |= first && none;
+    if (none || (!first && t <= LAZY)) t = 0.f;
+    const float a = __builtin_amdgcn_exp2f(-fmaxf(t, 0.f));   // (a first reference below 0: there is nothing to scale yet)
+    x.l[qt] *= a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) negm[qt][i] -= t;
+    asm volatile("" : "+v"(negm[qt]), "+v"(x.l[qt]));
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      x.s[kt][qt] -= t;
+      asm volatile("" : "+v"(x.s[kt][qt]));
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {   // one tile at a time, in the accumulator file before and after
+      asm volatile("" : "+a"(x.accO[dt][qt]));
+      x.accO[dt][qt] *= a;
+      asm volatile("" : "+a"(x.accO[dt][qt]));
+    }
+  }
+  return __any(open);
+}
+
+// the tiles of a list: addresses of the one to fetch next, and how many keys the tiles in flight hold.  All of it is the same for the whole wave and has to
+// live in scalar registers (`uni`, and the list behind a constant-address-space pointer: scalar loads)
+struct SpList {
+  const __attribute__((address_space(4))) int* p;
+  int pos, last;                                   // the entry to load, the list's last one (loaded again behind it)
+  int nxt;                                         // the entry that is fetched next
+  const char *kb, *vb;
+  uint32_t rs2;
+  int len, nvalid;
+  const char *ka, *va;                             // of the tile being fetched
+  uint32_t krec, vrec;
+  int rem0, rem1, rem2;                            // keys of tiles t, t + 1, t + 2
+};
+// nxt -> addresses; an entry that names no block: no keys, and nothing is read
+__device__ __forceinline__ void sp_apply_k(SpList& d) {
+  const bool ok = (uint32_t)d.nxt < (uint32_t)d.nvalid;
+  const int blk = ok ? d.nxt : 0;
+  d.rem2 = ok ? d.len - blk * KVBLK : 0;
+  d.ka = d.kb + (uint64_t)(uint32_t)blk * (uint64_t)(KVBLK * d.rs2);
+  const int rows = d.rem2 < KVBLK ? d.rem2 : KVBLK;
+  d.krec = ok ? (uint32_t)(rows - 1) * d.rs2 + 256u : 0u;   // rows past the last key read as zeros
+}
+__device__ __forceinline__ void sp_apply_v(SpList& d) {
+  const bool ok = (uint32_t)d.nxt < (uint32_t)d.nvalid;
+  d.va = d.vb + (uint64_t)(uint32_t)(ok ? d.nxt : 0) * (KVBLK * 2);
+  d.vrec = ok ? 0xfffffff0u : 0u;   // (all ones and 0 would be a sign extension of the condition, which hipcc makes in vector registers)
+}
+__device__ __forceinline__ void sp_load(SpList& d) {
+  d.nxt = d.p[d.pos < d.last ? d.pos : d.last];
+  d.pos += 1;
+}
+
+// The 16 DMA pieces of a wave for one tile, K and V^T in turn: 4 LDS rows of K (source rows permuted), 8 of V^T.  A piece of V^T is a
+// lane offset and a scalar one; those of K, whose rows past the last key have to fail the range check, are lane offsets as a whole
+struct SpDma {
+  uint32_t kofs[8], vofs, lds0, ldv2;
+};
+template <int AT>   // LDS bytes behind lds0 (added on the way into m0: forty such sums kept in scalar registers did not fit)
+__device__ __forceinline__ void sp_dma(uint32_t voff, const char* base, uint32_t num_records, uint32_t soff, uint32_t lds0) {
+  const uint64_t b = (uint64_t)base;
+  dma_u4 r;
+  r[0] = (uint32_t)b;
+  r[1] = (uint32_t)(b >> 32) & 0xffffu;  // stride 0
+  r[2] = num_records;                    // bytes from base that may be read; beyond: zeros
+  r[3] = 0x00020000u;
+  asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "s"(lds0), "n"(AT) : "memory", "scc");
+}
+template <int KS, int VS, int I>
+__device__ __forceinline__ void sp_piece(const SpDma& m, const SpList& d) {
+  constexpr int q = I >> 1;   // K: LDS rows 8 q .. 8 q + 7 (both waves); V^T: rows 16 q .. 16 q + 15
+  if constexpr ((I & 1) == 0) sp_dma<KS * IMG + q * 2048>(m.kofs[q], d.ka, d.krec, 0u, m.lds0);
+  else sp_dma<(2 + VS) * IMG + q * 2048>(m.vofs, d.va, d.vrec, (uint32_t)(16 * q) * m.ldv2, m.lds0);
+}
+template <int KS, int VS, int I = 0>
+__device__ __forceinline__ void sp_fetch(const SpDma& m, const SpList& d) {
+  if constexpr (I < 16) {
+    sp_piece<KS, VS, I>(m, d);
+    sp_fetch<KS, VS, I + 1>(m, d);
+  }
+}
+
+// the keys of a tile past the end: their V may hold anything, and 0 * anything has to be 0 (a tile without keys was filled with zeros)
+__device__ __forceinline__ void sp_clean(char* img, int rem, int wave) {
+  const int tid = wave * 64 + (int)sp_lane();
+#pragma unroll 1
+  for (int i = tid; i < 1024; i += 128) {
+    const int row = i >> 3, lim = rem - (((i & 7) ^ ((row >> 1) & 7)) * 8);   // keys of this 16-byte chunk that stay
+    u32x4* v = reinterpret_cast<u32x4*>(img + i * 16);
+    u32x4 w = *v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = lim >= 2 * j + 2 ? w[j] : lim == 2 * j + 1 ? w[j] & 0xffffu : 0u;
+    *v = w;
+  }
+  __syncthreads();
+}
+
+// the MFMA of gap G and what sits behind it; KS, VS: the images of tile t (K read already, V^T read here)
+template <int KS, int VS, int G>
+__device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], const int (&vaddr)[2], const mfma_bf16x8 (&qf)[4][4], f32x4 (&negm)[4], mfma_bf16x8 (&kf)[4][4],
+                                        mfma_bf16x8 (&vf)[8][2], SHalf& a, SHalf& b, const SpDma& m, SpList& d, bool& force_a, bool& force_b) {
+  constexpr int KN = (KS ^ 1) * IMG, VB = (2 + VS) * IMG;
+  if constexpr (G < 32) sp_s_step(a, kf, qf, negm, 0, G);
+  else if constexpr (G < 64) sp_pv_step(b, vf, G - 32);
+  else if constexpr (G < 96) sp_s_step(b, kf, qf, negm, 2, G - 64);
+  else sp_pv_step(a, vf, G - 96);
+  SB();
+  if constexpr ((G & 1) == 0) {
+    if constexpr (G <= 42) sp_exp(b, 10 + G / 2);
+    else if constexpr (G <= 106) sp_exp(a, (G - 44) / 2);
+    else sp_exp(b, (G - 108) / 2);
+    if constexpr (G == 0) sp_apply_k(d);
+    if constexpr (G == 2) sp_load(d);
+  } else {
+    // behind an odd score: its pair's pack; behind an even one: the sum of the pair before
+    constexpr int K = G <= 43 ? 10 + G / 2 : G <= 107 ? (G - 45) / 2 : (G - 109) / 2;
+    SHalf& x = G > 43 && G <= 107 ? a : b;
+    if constexpr ((K & 1) == 1) sp_pack(x, K);
+    else if constexpr (K > 0) sp_sum(x, K - 1);
+    else if constexpr (G == 45) sp_sum(b, 31);
+    else sp_sum(a, 31);
+    if constexpr (G >= 41 && G <= 55) vf[(G - 41) / 2][0] = *(lds_frag*)(lds + (VB + (G - 41) / 2 * 2048) + vaddr[0]);
+    if constexpr (G >= 57 && G <= 71) vf[(G - 57) / 2][1] = *(lds_frag*)(lds + (VB + (G - 57) / 2 * 2048) + vaddr[1]);
+    if constexpr (G >= 67 && G <= 97) {
+      constexpr int R = (G - 67) / 2;
+      kf[R & 3][R >> 2] = *(lds_frag*)(lds + (KN + (R & 3) * 4096) + kaddr[R >> 2]);
+    }
+    if constexpr (G == 1) sp_apply_v(d);
+    if constexpr (G >= 3 && G <= 33) sp_piece<KS, (VS + 2) % 3, (G - 3) / 2>(m, d);
+    if constexpr (G >= 29 && G <= 43) {
+      sp_max<(G - 29) / 2>(a, 0);
+      sp_max<(G - 29) / 2>(a, 1);
+    }
+    if constexpr (G >= 93 && G <= 107) {
+      sp_max<(G - 93) / 2>(b, 0);
+      sp_max<(G - 93) / 2>(b, 1);
+    }
+    if constexpr (G == 43) {
+      if (__builtin_expect(force_a || d.rem0 < KVBLK || __any(fmaxf(a.top[0], a.top[1]) > LAZY), 0)) {
+        asm volatile("" ::: "memory");
+        force_a = sp_cold(a, &negm[0], d.rem0);
+      }
+    }
+    if constexpr (G == 107) {
+      if (__builtin_expect(force_b || d.rem0 < KVBLK || __any(fmaxf(b.top[0], b.top[1]) > LAZY), 0)) {
+        asm volatile("" ::: "memory");
+        force_b = sp_cold(b, &negm[2], d.rem0);
+      }
+    }
+  }
+  SB();
+  if constexpr (G < 127) sp_slot<KS, VS, G + 1>(lds, kaddr, vaddr, qf, negm, kf, vf, a, b, m, d, force_a, force_b);
+}
+
 struct SparseArgs {
   const bf16_t *q, *k, *vt;
   bf16_t* o;
@@ -22,207 +277,228 @@ struct SparseArgs {
   const int *index, *count, *k_lens;
   int B, Bk, H, Hk, nq, keep;
   int q_prescaled;
+  int parts;
+  float* part;    // parts > 1: [list][part][128 rows][128] sums, behind them [list][part][128 rows] {reference, row sum}
 };
 
-__device__ __forceinline__ f32x4 mfma16(const mfma_bf16x8& a, const mfma_bf16x8& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// 4 waves x 32 queries, one list entry at a time, two stages of K / V^T in LDS
-__global__ __launch_bounds__(256, 2) void attn_sparse_kernel(SparseArgs p) {
-  __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // K stage 0, 1, V^T stage 0, 1
+// PARTS: a list is cut into `parts` workgroups' shares, which leave unnormalised sums for sparse_join_kernel
+template <bool PARTS>
+__global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[5 * IMG];   // K 0, 1, V^T 0, 1, 2
   lds_cchar* lds = (lds_cchar*)smem;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int wg = xcd_remap(blockIdx.x, gridDim.x);   // an XCD gets runs of neighbouring blocks of queries of a head: their lists have much in common
+  const int id = PARTS ? wg / p.parts : wg, pt = PARTS ? wg - id * p.parts : 0;
   const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
   const int bk = b % p.Bk, hk = h / (p.H / p.Hk);
-  const int* list = p.index + (int64_t)id * p.keep;
+
+  typedef const __attribute__((address_space(4))) int const_int;
   int entries = p.keep;
-  if (p.count != nullptr) entries = min(entries, max(p.count[id], 0));
+  if (p.count != nullptr) entries = min(entries, max(((const_int*)p.count)[id], 0));
   int len = (int)p.Lk;
-  if (p.k_lens != nullptr) len = min(len, max(p.k_lens[bk], 0));
-  const int nvalid = (len + KVBLK - 1) / KVBLK;
-  const char* kb = reinterpret_cast<const char*>(p.k + (int64_t)bk * p.k_batch + (int64_t)hk * 128);
-  const char* vb = reinterpret_cast<const char*>(p.vt + ((int64_t)bk * p.Hk + hk) * 128 * p.ldv);
-  const uint32_t rs2 = (uint32_t)(p.k_row * 2), ldv2 = (uint32_t)(p.ldv * 2);
-
-  uint32_t kofs[4], vofs[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t m = (uint32_t)tid >> 4;
-    kofs[i] = (32u * (i >> 1) + 8u * (m >> 2) + 4u * (i & 1) + (m & 3u)) * rs2 + (((uint32_t)tid & 15u) ^ m) * 16u;
-    vofs[i] = (32u * i + ((uint32_t)tid >> 3)) * ldv2 + ((((uint32_t)tid & 7u) ^ (((uint32_t)tid >> 4) & 7u)) << 4);
+  if (p.k_lens != nullptr) len = min(len, max(((const_int*)p.k_lens)[bk], 0));
+  SpList d;
+  d.len = uni(len);
+  d.nvalid = uni((len + KVBLK - 1) / KVBLK);
+  int e0 = 0, e1 = entries;
+  if (PARTS) {
+    e0 = (int)((int64_t)entries * pt / p.parts);
+    e1 = (int)((int64_t)entries * (pt + 1) / p.parts);
   }
-  auto fetch = [&](int blk, int st) {
-    blk = __builtin_amdgcn_readfirstlane(blk);
-    const int rows = min(KVBLK, len - blk * KVBLK);
-    const char* ka = uni(kb + (int64_t)blk * KVBLK * rs2);
-    const char* va = uni(vb + (int64_t)blk * KVBLK * 2);
-    const uint32_t klen = uni((uint32_t)(rows - 1) * rs2 + 256u);     // rows past the last key read as zeros
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      dma_issue(kofs[i], ka, klen, lds0 + st * IMG + wave * 1024 + i * 4096);
-      dma_issue(vofs[i], va, 0xffffffffu, lds0 + (2 + st) * IMG + wave * 1024 + i * 4096);
-    }
-  };
-  // the next entry that names a block with keys, from position e on
-  auto next = [&](int e) {
-    while (e < entries && (unsigned)list[e] >= (unsigned)nvalid) ++e;
-    return e;
-  };
+  const int nt = d.nvalid > 0 ? uni(e1 - e0) : 0;
 
-  const int64_t q0 = (int64_t)qb * Q_BLOCK + wave * 32;
-  mfma_bf16x8 qf[2][4];
+  const int64_t q0 = (int64_t)qb * Q_BLOCK + wave * 64;
+  SHalf x[2];
+  f32x4 negm[4];
 #pragma unroll
-  for (int qt = 0; qt < 2; ++qt) {
-    const int64_t r = min(q0 + 16 * qt + n, p.Lq - 1);
-    const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
-      if (!p.q_prescaled) {   // the scale folded into q and rounded with it (as the dense kernels do): no multiplication per score
-        float f[8];
-        unpack8(w, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
-        w = pack8(f);
-      }
-      qf[qt][ks] = __builtin_bit_cast(mfma_bf16x8, w);
-    }
-  }
-  const uint4 one_bits = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  const mfma_bf16x8 ones = __builtin_bit_cast(mfma_bf16x8, one_bits);
-  f32x4 acc[8][2], l[2], negm[2];
-#pragma unroll
-  for (int qt = 0; qt < 2; ++qt) {
-    l[qt] = negm[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) acc[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  bool unset[2] = {true, true};   // the row has no reference yet
-
-  int e = next(0), st = 0;
-  if (e < entries) fetch(list[e], 0);
-  bool force = true;
-  while (e < entries) {
-    const int blk = __builtin_amdgcn_readfirstlane(list[e]);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    e = next(e + 1);
-    if (e < entries) fetch(list[e], st ^ 1);
-    const int rem = len - blk * KVBLK;
-    if (rem < KVBLK) {   // the keys past the end: their V may hold anything, 0 * anything has to be 0
-      for (int i = tid; i < 1024; i += 256) {
-        const int row = i >> 3, lim = rem - (((i & 7) ^ ((row >> 1) & 7)) * 8);
-        bf16_t* v = reinterpret_cast<bf16_t*>(smem + (2 + st) * IMG + i * 16);
-        for (int j = max(lim, 0); j < 8; ++j) v[j] = 0;
-      }
-      __syncthreads();
-    }
-    // S - m: the reference enters as the C operand of each tile's first product
-    f32x4 s[4][2];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const mfma_bf16x8 kf = *(lds_frag*)(lds + st * IMG + (16 * kt + n) * 256 + (((4 * ks + g) ^ n) << 4));
-        s[kt][0] = mfma16(kf, qf[0][ks], ks == 0 ? negm[0] : s[kt][0]);
-        s[kt][1] = mfma16(kf, qf[1][ks], ks == 0 ? negm[1] : s[kt][1]);
-      }
-    if (rem < KVBLK) {
-#pragma unroll
-      for (int qt = 0; qt < 2; ++qt)
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + i >= rem) s[kt][qt][i] = -INFINITY;
-    }
-    float top[2];
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
-      top[qt] = fmaxf(s[0][qt][0], s[0][qt][1]);
+      negm[2 * c + qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[c].l[qt] = 0.f;
+      x[c].top[qt] = 0.f;
 #pragma unroll
-      for (int k = 2; k < 16; k += 2) top[qt] = fmaxf(top[qt], fmaxf(s[k >> 2][qt][k & 3], s[(k + 1) >> 2][qt][(k + 1) & 3]));
-    }
-    // The reference m of a row follows its maximum only when a score lies more than 2^LAZY above it: until then the weights 2^(s - m) are merely
-    // large numbers, which bf16 and fp32 carry with the same relative precision.  The first block sets it.
-    if (force || __any(fmaxf(top[0], top[1]) > LAZY)) {
-      bool open = false;
-#pragma unroll
-      for (int qt = 0; qt < 2; ++qt) {
-        float t = top[qt];
-        t = fmaxf(t, __shfl_xor(t, 16, 64));
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        const bool none = t == -INFINITY;      // (every product so far is -inf: the row waits for a block with another)
-        if (none || (!unset[qt] && t <= LAZY)) t = 0.f;
-        unset[qt] = unset[qt] && none;
-        open |= unset[qt];
-        const float a = __builtin_amdgcn_exp2f(-t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { negm[qt][i] -= t; l[qt][i] *= a; }
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) acc[dt][qt] *= a;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[kt][qt][i] -= t;
+      for (int dt = 0; dt < 8; ++dt) {
+        x[c].accO[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        asm volatile("" : "+a"(x[c].accO[dt][qt]));
       }
-      force = __any(open);
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) x[c].s[kt][qt] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (b's weights "of the tile before" the first: zeros)
     }
-    mfma_bf16x8 pf[2][2];
+    x[c].p0 = x[c].p1 = 0.f;
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt)
+    for (int f = 0; f < 4; ++f) x[c].pk[f] = u32x4{0u, 0u, 0u, 0u};
+  }
+  if (nt > 0) {
+    d.p = (const_int*)(p.index + (int64_t)id * p.keep + e0);
+    d.last = nt - 1;
+    d.pos = 0;
+    d.rs2 = uni((uint32_t)(p.k_row * 2));
+    d.kb = uni(reinterpret_cast<const char*>(p.k + (int64_t)bk * p.k_batch + (int64_t)hk * 128));
+    d.vb = uni(reinterpret_cast<const char*>(p.vt + ((int64_t)bk * p.Hk + hk) * 128 * p.ldv));
+    SpDma m;
+    m.lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 1024;
+    m.ldv2 = uni((uint32_t)(p.ldv * 2));
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint4 w;
-        w.x = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c][qt][0]), __builtin_amdgcn_exp2f(s[2 * c][qt][1]));
-        w.y = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c][qt][2]), __builtin_amdgcn_exp2f(s[2 * c][qt][3]));
-        w.z = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c + 1][qt][0]), __builtin_amdgcn_exp2f(s[2 * c + 1][qt][1]));
-        w.w = cvt_pk(__builtin_amdgcn_exp2f(s[2 * c + 1][qt][2]), __builtin_amdgcn_exp2f(s[2 * c + 1][qt][3]));
-        pf[qt][c] = __builtin_bit_cast(mfma_bf16x8, w);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t r = 8u * (i & 1) + ((uint32_t)tid >> 4), kt = i >> 1;   // LDS row 16 kt + r
+      m.kofs[i] = (32u * (kt >> 1) + 8u * (r >> 2) + 4u * (kt & 1) + (r & 3u)) * d.rs2 + (((uint32_t)tid & 15u) ^ r) * 16u;
+    }
+    m.vofs = ((uint32_t)tid >> 3) * m.ldv2 + ((((uint32_t)tid & 7u) ^ (((uint32_t)tid >> 4) & 7u)) << 4);
+    sp_load(d); sp_apply_k(d); sp_apply_v(d);
+    d.rem0 = d.rem2;
+    sp_fetch<0, 0>(m, d);
+    sp_load(d); sp_apply_k(d); sp_apply_v(d);
+    d.rem1 = d.rem2;
+    sp_fetch<1, 1>(m, d);
+    sp_load(d);
+
+    mfma_bf16x8 qf[4][4], kf[4][4], vf[8][2];
+#pragma unroll
+    for (int qt = 0; qt < 4; ++qt) {
+      const int64_t r = min(q0 + 16 * qt + n, p.Lq - 1);
+      const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
+        if (!p.q_prescaled) {   // the scale folded into q and rounded with it (as the dense kernels do): no multiplication per score
+          float f[8];
+          unpack8(w, f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
+          w = pack8(f);
+        }
+        qf[qt][ks] = __builtin_bit_cast(mfma_bf16x8, w);
+        asm volatile("" : "+a"(qf[qt][ks]));
       }
-    // the row sums are one more tile of the product, over a V of ones: of the rounded weights, as the numerator's, and already over all lanes
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      l[0] = mfma16(ones, pf[0][c], l[0]);
-      l[1] = mfma16(ones, pf[1][c], l[1]);
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int row = 16 * dt + n;
-        const mfma_bf16x8 vf = *(lds_frag*)(lds + (2 + st) * IMG + row * 128 + (((4 * c + g) ^ ((row >> 1) & 7)) << 4));
-        acc[dt][0] = mfma16(vf, pf[0][c], acc[dt][0]);
-        acc[dt][1] = mfma16(vf, pf[1][c], acc[dt][1]);
+        vf[dt][c] = __builtin_bit_cast(mfma_bf16x8, make_uint4(0u, 0u, 0u, 0u));
+        asm volatile("" : "+a"(vf[dt][c]));
       }
-    st ^= 1;
-  }
+    int kaddr[4], vaddr[2];
 #pragma unroll
-  for (int qt = 0; qt < 2; ++qt) {
-    const float t = l[qt][0];
-    const float inv = t == 0.f ? 0.f : 1.f / t;   // a row without keys: zeros
-    const int64_t r = q0 + 16 * qt + n;
-    if (r < p.Lq) {
-      bf16_t* op = p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 4 * g;
+    for (int ks = 0; ks < 4; ++ks) kaddr[ks] = n * 256 + (((4 * ks + g) ^ n) << 4);
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) {
-        uint2 w;
-        w.x = cvt_pk(acc[dt][qt][0] * inv, acc[dt][qt][1] * inv);
-        w.y = cvt_pk(acc[dt][qt][2] * inv, acc[dt][qt][3] * inv);
-        *reinterpret_cast<uint2*>(op + 16 * dt) = w;
+    for (int c = 0; c < 2; ++c) vaddr[c] = n * 128 + (((4 * c + g) ^ ((n >> 1) & 7)) << 4);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < 16; ++r) kf[r & 3][r >> 2] = *(lds_frag*)(lds + (r & 3) * 4096 + kaddr[r >> 2]);
+
+    bool force_a = true, force_b = true;
+#define SP_TILE(J)                                                                                                               \
+    if (t + (J) >= nt) break;                                                                                                    \
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   /* tile t + 1 has landed, tile t - 1 is read */                 \
+    __builtin_amdgcn_s_barrier();                                                                                                \
+    asm volatile("" ::: "memory");                                                                                               \
+    if (__builtin_expect(d.rem0 < KVBLK, 0)) sp_clean(smem + (2 + (J) % 3) * IMG, d.rem0, wave);                                  \
+    sp_slot<(J) & 1, (J) % 3, 0>(lds, kaddr, vaddr, qf, negm, kf, vf, x[0], x[1], m, d, force_a, force_b);                        \
+    d.rem0 = d.rem1;                                                                                                             \
+    d.rem1 = d.rem2;
+    for (int t = 0;; t += 6) {
+      SP_TILE(0)
+      SP_TILE(1)
+      SP_TILE(2)
+      SP_TILE(3)
+      SP_TILE(4)
+      SP_TILE(5)
+    }
+#undef SP_TILE
+    // b's last weights and products
+    sp_sum(x[1], 9);
+#pragma unroll
+    for (int k = 10; k < 32; ++k) {
+      sp_exp(x[1], k);
+      if (k & 1) {
+        asm volatile("s_nop 1");   // (no MFMA between the exp2 and its use here)
+        sp_pack(x[1], k);
+        sp_sum(x[1], k);
       }
     }
+    asm volatile("s_nop 7" ::: "memory");
+    SB();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) { sp_pv_step(x[1], vf, i); SB(); }
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");   // trailing DMA (the LDS is released at the end); the last MFMAs -> accumulator reads
   }
+  const int lane_e = (int)sp_lane(), ne = lane_e & 15, ge = lane_e >> 4;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      const int row = wave * 64 + 32 * c + 16 * qt + ne;
+      float l = x[c].l[qt];
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      if (PARTS) {
+        float* o = p.part + ((int64_t)wg * Q_BLOCK + row) * 128 + 4 * ge;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<float4*>(o + 16 * dt) = make_float4(x[c].accO[dt][qt][0], x[c].accO[dt][qt][1], x[c].accO[dt][qt][2], x[c].accO[dt][qt][3]);
+        if (ge == 0) {
+          float2* st = reinterpret_cast<float2*>(p.part + (int64_t)gridDim.x * Q_BLOCK * 128) + (int64_t)wg * Q_BLOCK + row;
+          *st = make_float2(l == 0.f ? -INFINITY : -negm[2 * c + qt][0], l);
+        }
+        continue;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;   // a row without keys: zeros
+      if ((int64_t)qb * Q_BLOCK + row < p.Lq) {
+        bf16_t* op = p.o + ((int64_t)b * p.Lq + (int64_t)qb * Q_BLOCK + row) * p.H * 128 + (int64_t)h * 128 + 4 * ge;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          uint2 w;
+          w.x = cvt_pk(x[c].accO[dt][qt][0] * inv, x[c].accO[dt][qt][1] * inv);
+          w.y = cvt_pk(x[c].accO[dt][qt][2] * inv, x[c].accO[dt][qt][3] * inv);
+          *reinterpret_cast<uint2*>(op + 16 * dt) = w;
+        }
+      }
+    }
+}
+
+// o = sum of the parts' sums, each scaled from its own reference to the largest, over the row sums likewise: 8 rows x 32 lanes of four columns
+__global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs) {
+  const int id = blockIdx.x, row = blockIdx.y * 8 + (threadIdx.x >> 5), c = threadIdx.x & 31;
+  const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
+  const int64_t r = (int64_t)qb * Q_BLOCK + row;
+  if (r >= p.Lq) return;
+  const float* o = p.part + ((int64_t)id * p.parts * Q_BLOCK + row) * 128 + 4 * c;
+  const float2* st = reinterpret_cast<const float2*>(p.part + (int64_t)wgs * Q_BLOCK * 128) + (int64_t)id * p.parts * Q_BLOCK + row;
+  float top = -INFINITY;
+  for (int k = 0; k < p.parts; ++k) top = fmaxf(top, st[k * Q_BLOCK].x);
+  float s[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  if (top != -INFINITY) {
+    for (int k = 0; k < p.parts; ++k) {
+      const float2 ml = st[k * Q_BLOCK];
+      const float4 v = *reinterpret_cast<const float4*>(o + (int64_t)k * Q_BLOCK * 128);
+      const float a = __builtin_amdgcn_exp2f(ml.x - top);
+      l += ml.y * a;
+      s[0] += v.x * a; s[1] += v.y * a; s[2] += v.z * a; s[3] += v.w * a;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 4 * c) = make_uint2(cvt_pk(s[0] * inv, s[1] * inv), cvt_pk(s[2] * inv, s[3] * inv));
+}
+
+// how many workgroups share a list: enough for two on every CU, a share no shorter than SPARSE_MIN_SHARE blocks
+int sparse_parts(int64_t lists, int keep) {
+  int64_t n = 512 / lists;
+  if (n > keep / 2) n = keep / 2;
+  if (n > 32) n = 32;
+  return n < 2 ? 1 : (int)n;
 }
 
 }  // namespace
 
 extern "C" int64_t wan_sparse_attention_scratch_bytes(int B, int64_t Lq, int H, int keep) {
-  return 0;
+  if (B < 1 || Lq < 1 || H < 1 || keep < 1) return 0;
+  const int64_t lists = (Lq + Q_BLOCK - 1) / Q_BLOCK * H * B;
+  const int parts = sparse_parts(lists, keep);
+  return parts == 1 ? 0 : lists * parts * Q_BLOCK * (128 + 2) * 4;
 }
 
 extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_batch, const wan_bf16* k, int64_t k_row, int64_t k_batch, const wan_bf16* vt, wan_bf16* o,
@@ -240,8 +516,19 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   WAN_REQUIRE(k_row < ((int64_t)1 << 24) && ldv < ((int64_t)1 << 23), "wan_sparse_attention: a row of k of %lld elements or %lld keys exceed the kernel's offsets", (long long)k_row, (long long)ldv);
   const int64_t nq = (Lq + Q_BLOCK - 1) / Q_BLOCK;
   WAN_REQUIRE(nq * H * B < ((int64_t)1 << 31), "wan_sparse_attention: grid too large");
-  SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled};
-  hipLaunchKernelGGL(attn_sparse_kernel, dim3((unsigned)(nq * H * B)), dim3(256), 0, as_stream(stream), a);
+  const int64_t lists = nq * H * B;
+  const int parts = sparse_parts(lists, keep);
+  const int64_t need = wan_sparse_attention_scratch_bytes(B, Lq, H, keep);
+  WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_sparse_attention: needs 16-byte aligned scratch of %lld bytes", (long long)need);
+  hipStream_t st = as_stream(stream);
+  const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, parts, reinterpret_cast<float*>(scratch)};
+  if (parts == 1) {
+    hipLaunchKernelGGL(attn_sparse_kernel<false>, dim3((unsigned)lists), dim3(128), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(attn_sparse_kernel<true>, dim3((unsigned)(lists * parts)), dim3(128), 0, st, a);
+    const int64_t rows = Lq < Q_BLOCK ? Lq : Q_BLOCK;
+    hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)lists, (unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, (int)(lists * parts));
+  }
   WAN_LAUNCH_CHECK();
   return 0;
 }
