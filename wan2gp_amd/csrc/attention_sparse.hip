@@ -23,11 +23,12 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     two images and V^T in one of three (K(t) is in registers by the time K(t + 2) is fetched, V^T(t) is read in the middle of tile t);
 //   * the tiles' addresses come from the list, one scalar load a tile ahead of its use;
 //   * the softmax needs no bound on the scores: a half's maximum is taken (v_max3) between its last S tile and its first exp2, and only a score 2^LAZY
-//     above the row's reference, the first tile and tiles that end inside leave the straight path (cold16);
-//   * row sums by v_dot2_f32_bf16 over the packed pairs: one instruction for two scores, and of the rounded weights, as the product's.
-// Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 44 + 2 k, of b's behind 108 + 2 k, running into the next tile (k = 10 behind its
-// MFMA 0); a pair is packed in the odd gap behind its second exp2 and summed one odd gap later; maxima of a in the odd gaps 29 .. 43, of b 93 .. 107; DMA of tile
-// t + 2 in the odd gaps 3 .. 33; V^T(t) fragments 41 .. 71, K(t + 1) fragments 67 .. 97.
+//     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
+// Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
+// MFMA 0); a score is summed in the odd gap behind the next one's exp2, a pair packed in the odd gap behind its second; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
+// t + 2 in every eighth gap, K from 3, V^T from 65 (the m0 of each in the gap in front of it): 64 pieces of 1 KB a CU and tile keep the path into the LDS
+// busy for 1,024 cycles, and issued in a row they hold up the waves; V^T(t) fragments 41 .. 71, K(t + 1) fragments 67 .. 97; the
+// addresses of tile t + 3 in the even gaps 112 .. 124.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct SHalf {
   f32x4 accO[8][2];   // O^T tiles [d tile][q tile]
@@ -61,19 +62,20 @@ __device__ __forceinline__ float sp_score(const SHalf& x, int k) {
   return x.s[2 * (f >> 1) + ((k >> 2) & 1)][f & 1][k & 3];
 }
 __device__ __forceinline__ void sp_exp(SHalf& x, int k) {
-  // (asm: behind the builtin hipcc puts an s_nop in front of the pack, not counting the MFMA that stands between as the wait state it is)
-  if (k & 1) asm volatile("v_exp_f32 %0, %1" : "=v"(x.p1) : "v"(sp_score(x, k)));
-  else asm volatile("v_exp_f32 %0, %1" : "=v"(x.p0) : "v"(sp_score(x, k)));
+  float& p = (k & 1) ? x.p1 : x.p0;
+  p = __builtin_amdgcn_exp2f(sp_score(x, k));
+  asm volatile("" : "+v"(p));
 }
 __device__ __forceinline__ void sp_pack(SHalf& x, int k) {   // behind the odd score k
   const int j = k >> 1;
   x.pk[j >> 2][j & 3] = cvt_pk(x.p0, x.p1);
   asm volatile("" : "+v"(x.pk[j >> 2]));
 }
-__device__ __forceinline__ void sp_sum(SHalf& x, int k) {    // the pair that ends with the odd score k
-  const int j = k >> 1, qt = (k >> 3) & 1;
-  const uint32_t pair = x.pk[j >> 2][j & 3];   // (a value of its own: bit_cast of a vector's element takes element 0)
-  x.l[qt] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(hw_bf16x2, pair), __builtin_bit_cast(hw_bf16x2, 0x3f803f80u), x.l[qt], false);
+// score k's weight into its row's sum: a plain add, in front of the pack of its gap -- a compiler's instruction there is the wait state that hipcc would otherwise fill
+// with an s_nop, not counting the asm MFMA.  (v_dot2_f32_bf16 over the packed pair is half as many instructions and cost 400 cycles a tile more.)
+__device__ __forceinline__ void sp_sum(SHalf& x, int k) {
+  const int qt = (k >> 3) & 1;
+  x.l[qt] += (k & 1) ? x.p1 : x.p0;
   asm volatile("" : "+v"(x.l[qt]));
 }
 // step j = 0 .. 7 of the maximum over a q tile's 16 scores, in the order the S tiles are finished
@@ -92,10 +94,19 @@ __device__ __forceinline__ uint32_t sp_lane() {
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
   return lane;
 }
+// step T = 0 .. 11 of both q tiles' maxima: one operation a gap while tiles are being finished, two from the ninth on
+template <int T>
+__device__ __forceinline__ void sp_maxes(SHalf& x) {
+  if constexpr (T < 8) sp_max<T / 2>(x, T & 1);
+  else {
+    sp_max<T - 4>(x, 0);
+    sp_max<T - 4>(x, 1);
+  }
+}
 // What leaves the straight path: the scores of a tile's keys past the end become -inf, and a row's reference moves to its maximum -- for the first
 // time (the row sum is 0: until a key has a finite score the reference is 0 and waits), or because a score lies more than 2^LAZY above it.
 // Returns whether a row still waits.
-__device__ __forceinline__ bool sp_cold(SHalf& x, f32x4* negm, int rem) {
+__device__ __forceinline__ int sp_cold(SHalf& x, f32x4* negm, int rem) {
   bool open = false;
   const int lim = rem - 8 * (int)(sp_lane() >> 4);
 #pragma unroll
@@ -134,7 +145,7 @@ __device__ __forceinline__ bool sp_cold(SHalf& x, f32x4* negm, int rem) {
       asm volatile("" : "+a"(x.accO[dt][qt]));
     }
   }
-  return __any(open);
+  return __any(open) ? 1 : 0;
 }
 
 // the tiles of a list: addresses of the one to fetch next, and how many keys the tiles in flight hold.  All of it is the same for the whole wave and has to
@@ -142,31 +153,42 @@ __device__ __forceinline__ bool sp_cold(SHalf& x, f32x4* negm, int rem) {
 struct SpList {
   const __attribute__((address_space(4))) int* p;
   int pos, last;                                   // the entry to load, the list's last one (loaded again behind it)
-  int nxt;                                         // the entry that is fetched next
+  int nxt;                                         // the entry loaded last
   const char *kb, *vb;
   uint32_t rs2;
   int len, nvalid;
-  const char *ka, *va;                             // of the tile being fetched
+  const char *ka, *va;                             // of the tile that is fetched next
   uint32_t krec, vrec;
-  int rem0, rem1, rem2;                            // keys of tiles t, t + 1, t + 2
+  int rem0, rem1, rem2, rem3;                      // keys of tiles t, t + 1, ..
+  int blk;
 };
-// nxt -> addresses; an entry that names no block: no keys, and nothing is read
-__device__ __forceinline__ void sp_apply_k(SpList& d) {
+// nxt -> addresses, in steps that fit the gaps of the tile before; an entry that names no block: no keys, and nothing is read.  (The empty asm statements keep
+// each step's result in scalar registers and in its gap: hipcc would otherwise do all of it, on the vector ALU, in front of the first use.)
+__device__ __forceinline__ void sp_apply_block(SpList& d) {
   const bool ok = (uint32_t)d.nxt < (uint32_t)d.nvalid;
-  const int blk = ok ? d.nxt : 0;
-  d.rem2 = ok ? d.len - blk * KVBLK : 0;
-  d.ka = d.kb + (uint64_t)(uint32_t)blk * (uint64_t)(KVBLK * d.rs2);
-  const int rows = d.rem2 < KVBLK ? d.rem2 : KVBLK;
-  d.krec = ok ? (uint32_t)(rows - 1) * d.rs2 + 256u : 0u;   // rows past the last key read as zeros
+  d.blk = ok ? d.nxt : 0;
+  d.rem3 = ok ? d.len - d.nxt * KVBLK : 0;      // (0 or more than 0: also what says whether the entry names a block)
+  asm volatile("" : "+s"(d.blk), "+s"(d.rem3));
+}
+__device__ __forceinline__ void sp_apply_k(SpList& d) {
+  d.ka = d.kb + (uint64_t)(uint32_t)d.blk * (uint64_t)(KVBLK * d.rs2);
+  asm volatile("" : "+s"(d.ka));
+}
+__device__ __forceinline__ void sp_apply_rows(SpList& d) {
+  const int rows = d.rem3 < KVBLK ? d.rem3 : KVBLK;
+  d.krec = d.rem3 > 0 ? (uint32_t)(rows - 1) * d.rs2 + 256u : 0u;   // rows past the last key read as zeros
+  asm volatile("" : "+s"(d.krec));
 }
 __device__ __forceinline__ void sp_apply_v(SpList& d) {
-  const bool ok = (uint32_t)d.nxt < (uint32_t)d.nvalid;
-  d.va = d.vb + (uint64_t)(uint32_t)(ok ? d.nxt : 0) * (KVBLK * 2);
-  d.vrec = ok ? 0xfffffff0u : 0u;   // (all ones and 0 would be a sign extension of the condition, which hipcc makes in vector registers)
+  d.va = d.vb + (uint64_t)(uint32_t)d.blk * (KVBLK * 2);
+  d.vrec = d.rem3 > 0 ? 0xfffffff0u : 0u;   // (all ones and 0 would be a sign extension of the condition, which hipcc makes in vector registers)
+  asm volatile("" : "+s"(d.va), "+s"(d.vrec));
 }
+__device__ __forceinline__ void sp_apply(SpList& d) { sp_apply_block(d); sp_apply_k(d); sp_apply_rows(d); sp_apply_v(d); }
 __device__ __forceinline__ void sp_load(SpList& d) {
   d.nxt = d.p[d.pos < d.last ? d.pos : d.last];
   d.pos += 1;
+  asm volatile("" : "+s"(d.pos));
 }
 
 // The 16 DMA pieces of a wave for one tile, K and V^T in turn: 4 LDS rows of K (source rows permuted), 8 of V^T.  A piece of V^T is a
@@ -174,26 +196,34 @@ __device__ __forceinline__ void sp_load(SpList& d) {
 struct SpDma {
   uint32_t kofs[8], vofs, lds0, ldv2;
 };
-template <int AT>   // LDS bytes behind lds0 (added on the way into m0: forty such sums kept in scalar registers did not fit)
-__device__ __forceinline__ void sp_dma(uint32_t voff, const char* base, uint32_t num_records, uint32_t soff, uint32_t lds0) {
+// Two statements: the LDS address goes into m0 a gap ahead (nothing that hipcc emits in a tile touches m0; together they need an s_nop between them).  The
+// sum is made on the way into m0: forty of them kept in scalar registers did not fit.
+template <int KS, int VS, int I>
+__device__ __forceinline__ void sp_m0(const SpDma& m) {
+  constexpr int q = I >> 1, AT = (I & 1) == 0 ? KS * IMG + q * 2048 : (2 + VS) * IMG + q * 2048;   // K: LDS rows 8 q .. 8 q + 7 (both waves); V^T: rows 16 q .. 16 q + 15
+  asm volatile("s_add_u32 m0, %0, %1" ::"s"(m.lds0), "n"(AT) : "scc", "memory");
+}
+__device__ __forceinline__ void sp_dma(uint32_t voff, const char* base, uint32_t num_records, uint32_t soff) {
   const uint64_t b = (uint64_t)base;
   dma_u4 r;
   r[0] = (uint32_t)b;
   r[1] = (uint32_t)(b >> 32) & 0xffffu;  // stride 0
   r[2] = num_records;                    // bytes from base that may be read; beyond: zeros
   r[3] = 0x00020000u;
-  asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "s"(lds0), "n"(AT) : "memory", "scc");
+  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff) : "memory");
 }
-template <int KS, int VS, int I>
+template <int I>
 __device__ __forceinline__ void sp_piece(const SpDma& m, const SpList& d) {
-  constexpr int q = I >> 1;   // K: LDS rows 8 q .. 8 q + 7 (both waves); V^T: rows 16 q .. 16 q + 15
-  if constexpr ((I & 1) == 0) sp_dma<KS * IMG + q * 2048>(m.kofs[q], d.ka, d.krec, 0u, m.lds0);
-  else sp_dma<(2 + VS) * IMG + q * 2048>(m.vofs, d.va, d.vrec, (uint32_t)(16 * q) * m.ldv2, m.lds0);
+  constexpr int q = I >> 1;
+  if constexpr ((I & 1) == 0) sp_dma(m.kofs[q], d.ka, d.krec, 0u);
+  else sp_dma(m.vofs, d.va, d.vrec, (uint32_t)(16 * q) * m.ldv2);
 }
 template <int KS, int VS, int I = 0>
 __device__ __forceinline__ void sp_fetch(const SpDma& m, const SpList& d) {
   if constexpr (I < 16) {
-    sp_piece<KS, VS, I>(m, d);
+    sp_m0<KS, VS, I>(m);
+    asm volatile("s_nop 0");
+    sp_piece<I>(m, d);
     sp_fetch<KS, VS, I + 1>(m, d);
   }
 }
@@ -216,7 +246,7 @@ __device__ __forceinline__ void sp_clean(char* img, int rem, int wave) {
 // the MFMA of gap G and what sits behind it; KS, VS: the images of tile t (K read already, V^T read here)
 template <int KS, int VS, int G>
 __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], const int (&vaddr)[2], const mfma_bf16x8 (&qf)[4][4], f32x4 (&negm)[4], mfma_bf16x8 (&kf)[4][4],
-                                        mfma_bf16x8 (&vf)[8][2], SHalf& a, SHalf& b, const SpDma& m, SpList& d, bool& force_a, bool& force_b) {
+                                        mfma_bf16x8 (&vf)[8][2], SHalf& a, SHalf& b, const SpDma& m, SpList& d, int& force_a, int& force_b) {
   constexpr int KN = (KS ^ 1) * IMG, VB = (2 + VS) * IMG;
   if constexpr (G < 32) sp_s_step(a, kf, qf, negm, 0, G);
   else if constexpr (G < 64) sp_pv_step(b, vf, G - 32);
@@ -224,43 +254,44 @@ __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], c
   else sp_pv_step(a, vf, G - 96);
   SB();
   if constexpr ((G & 1) == 0) {
-    if constexpr (G <= 42) sp_exp(b, 10 + G / 2);
-    else if constexpr (G <= 106) sp_exp(a, (G - 44) / 2);
-    else sp_exp(b, (G - 108) / 2);
-    if constexpr (G == 0) sp_apply_k(d);
-    if constexpr (G == 2) sp_load(d);
+    if constexpr (G <= 50) sp_exp(b, 6 + G / 2);
+    else if constexpr (G <= 114) sp_exp(a, (G - 52) / 2);
+    else sp_exp(b, (G - 116) / 2);
+    if constexpr (G <= 58 && G % 8 == 2) sp_m0<KS, (VS + 2) % 3, G / 8 * 2>(m);
+    if constexpr (G >= 64 && G % 8 == 0) sp_m0<KS, (VS + 2) % 3, (G - 64) / 8 * 2 + 1>(m);
+    if constexpr (G == 34) sp_load(d);
+    if constexpr (G == 112) sp_apply_block(d);
+    if constexpr (G == 116) sp_apply_k(d);
+    if constexpr (G == 118) sp_apply_rows(d);
+    if constexpr (G == 124) sp_apply_v(d);
   } else {
-    // behind an odd score: its pair's pack; behind an even one: the sum of the pair before
-    constexpr int K = G <= 43 ? 10 + G / 2 : G <= 107 ? (G - 45) / 2 : (G - 109) / 2;
-    SHalf& x = G > 43 && G <= 107 ? a : b;
-    if constexpr ((K & 1) == 1) sp_pack(x, K);
-    else if constexpr (K > 0) sp_sum(x, K - 1);
-    else if constexpr (G == 45) sp_sum(b, 31);
+    // the sum of the score before; behind an odd score its pair's pack
+    constexpr int K = G <= 51 ? 6 + G / 2 : G <= 115 ? (G - 53) / 2 : (G - 117) / 2;
+    SHalf& x = G > 51 && G <= 115 ? a : b;
+    if constexpr (K > 0) sp_sum(x, K - 1);
+    else if constexpr (G == 53) sp_sum(b, 31);
     else sp_sum(a, 31);
+    if constexpr ((K & 1) == 1) sp_pack(x, K);
     if constexpr (G >= 41 && G <= 55) vf[(G - 41) / 2][0] = *(lds_frag*)(lds + (VB + (G - 41) / 2 * 2048) + vaddr[0]);
     if constexpr (G >= 57 && G <= 71) vf[(G - 57) / 2][1] = *(lds_frag*)(lds + (VB + (G - 57) / 2 * 2048) + vaddr[1]);
     if constexpr (G >= 67 && G <= 97) {
       constexpr int R = (G - 67) / 2;
       kf[R & 3][R >> 2] = *(lds_frag*)(lds + (KN + (R & 3) * 4096) + kaddr[R >> 2]);
     }
-    if constexpr (G == 1) sp_apply_v(d);
-    if constexpr (G >= 3 && G <= 33) sp_piece<KS, (VS + 2) % 3, (G - 3) / 2>(m, d);
-    if constexpr (G >= 29 && G <= 43) {
-      sp_max<(G - 29) / 2>(a, 0);
-      sp_max<(G - 29) / 2>(a, 1);
-    }
-    if constexpr (G >= 93 && G <= 107) {
-      sp_max<(G - 93) / 2>(b, 0);
-      sp_max<(G - 93) / 2>(b, 1);
-    }
-    if constexpr (G == 43) {
-      if (__builtin_expect(force_a || d.rem0 < KVBLK || __any(fmaxf(a.top[0], a.top[1]) > LAZY), 0)) {
+    if constexpr (G <= 59 && G % 8 == 3) sp_piece<G / 8 * 2>(m, d);
+    if constexpr (G >= 65 && G % 8 == 1) sp_piece<(G - 65) / 8 * 2 + 1>(m, d);
+    if constexpr (G >= 29 && G <= 51) sp_maxes<(G - 29) / 2>(a);
+    if constexpr (G >= 93 && G <= 115) sp_maxes<(G - 93) / 2>(b);
+    if constexpr (G == 51) {
+      const uint64_t need = __ballot(fmaxf(a.top[0], a.top[1]) > LAZY) | (uint64_t)(force_a | (d.rem0 < KVBLK));
+      if (__builtin_expect(need != 0, 0)) {
         asm volatile("" ::: "memory");
         force_a = sp_cold(a, &negm[0], d.rem0);
       }
     }
-    if constexpr (G == 107) {
-      if (__builtin_expect(force_b || d.rem0 < KVBLK || __any(fmaxf(b.top[0], b.top[1]) > LAZY), 0)) {
+    if constexpr (G == 115) {
+      const uint64_t need = __ballot(fmaxf(b.top[0], b.top[1]) > LAZY) | (uint64_t)(force_b | (d.rem0 < KVBLK));
+      if (__builtin_expect(need != 0, 0)) {
         asm volatile("" ::: "memory");
         force_b = sp_cold(b, &negm[2], d.rem0);
       }
@@ -288,10 +319,10 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   lds_cchar* lds = (lds_cchar*)smem;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wg = xcd_remap(blockIdx.x, gridDim.x);   // an XCD gets runs of neighbouring blocks of queries of a head: their lists have much in common
-  const int id = PARTS ? wg / p.parts : wg, pt = PARTS ? wg - id * p.parts : 0;
-  const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
-  const int bk = b % p.Bk, hk = h / (p.H / p.Hk);
+  const int wg = uni(xcd_remap(blockIdx.x, gridDim.x));   // an XCD gets runs of neighbouring blocks of queries of a head: their lists have much in common
+  const int id = PARTS ? uni(wg / p.parts) : wg, pt = PARTS ? wg - id * p.parts : 0;
+  const int bh = uni(id / p.nq), qb = id - bh * p.nq, b = uni(bh / p.H), h = bh - b * p.H;
+  const int bk = uni(b % p.Bk), hk = uni(h / (p.H / p.Hk));
 
   typedef const __attribute__((address_space(4))) int const_int;
   int entries = p.keep;
@@ -303,8 +334,8 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   d.nvalid = uni((len + KVBLK - 1) / KVBLK);
   int e0 = 0, e1 = entries;
   if (PARTS) {
-    e0 = (int)((int64_t)entries * pt / p.parts);
-    e1 = (int)((int64_t)entries * (pt + 1) / p.parts);
+    e0 = uni((int)((int64_t)entries * pt / p.parts));
+    e1 = uni((int)((int64_t)entries * (pt + 1) / p.parts));
   }
   const int nt = d.nvalid > 0 ? uni(e1 - e0) : 0;
 
@@ -346,13 +377,14 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       m.kofs[i] = (32u * (kt >> 1) + 8u * (r >> 2) + 4u * (kt & 1) + (r & 3u)) * d.rs2 + (((uint32_t)tid & 15u) ^ r) * 16u;
     }
     m.vofs = ((uint32_t)tid >> 3) * m.ldv2 + ((((uint32_t)tid & 7u) ^ (((uint32_t)tid >> 4) & 7u)) << 4);
-    sp_load(d); sp_apply_k(d); sp_apply_v(d);
-    d.rem0 = d.rem2;
+    sp_load(d); sp_apply(d);
+    d.rem0 = d.rem3;
     sp_fetch<0, 0>(m, d);
-    sp_load(d); sp_apply_k(d); sp_apply_v(d);
-    d.rem1 = d.rem2;
+    sp_load(d); sp_apply(d);
+    d.rem1 = d.rem3;
     sp_fetch<1, 1>(m, d);
-    sp_load(d);
+    sp_load(d); sp_apply(d);
+    d.rem2 = d.rem3;
 
     mfma_bf16x8 qf[4][4], kf[4][4], vf[8][2];
 #pragma unroll
@@ -391,16 +423,19 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) kf[r & 3][r >> 2] = *(lds_frag*)(lds + (r & 3) * 4096 + kaddr[r >> 2]);
 
-    bool force_a = true, force_b = true;
+    int force_a = 1, force_b = 1;   // a row without a reference is left
 #define SP_TILE(J)                                                                                                               \
     if (t + (J) >= nt) break;                                                                                                    \
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   /* tile t + 1 has landed, tile t - 1 is read */                 \
+    d.krec = uni(d.krec);                                         /* (carried around the loop hipcc puts them into vector registers) */ \
+    d.rem0 = uni(d.rem0);                                                                                                        \
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");   /* V^T(t), K(t + 1) have landed, V^T(t + 1) may fly; tile t - 1 is read */ \
     __builtin_amdgcn_s_barrier();                                                                                                \
     asm volatile("" ::: "memory");                                                                                               \
     if (__builtin_expect(d.rem0 < KVBLK, 0)) sp_clean(smem + (2 + (J) % 3) * IMG, d.rem0, wave);                                  \
     sp_slot<(J) & 1, (J) % 3, 0>(lds, kaddr, vaddr, qf, negm, kf, vf, x[0], x[1], m, d, force_a, force_b);                        \
     d.rem0 = d.rem1;                                                                                                             \
-    d.rem1 = d.rem2;
+    d.rem1 = d.rem2;                                                                                                             \
+    d.rem2 = d.rem3;
     for (int t = 0;; t += 6) {
       SP_TILE(0)
       SP_TILE(1)
@@ -411,15 +446,13 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     }
 #undef SP_TILE
     // b's last weights and products
-    sp_sum(x[1], 9);
+    sp_sum(x[1], 5);
 #pragma unroll
-    for (int k = 10; k < 32; ++k) {
+    for (int k = 6; k < 32; ++k) {
       sp_exp(x[1], k);
-      if (k & 1) {
-        asm volatile("s_nop 1");   // (no MFMA between the exp2 and its use here)
-        sp_pack(x[1], k);
-        sp_sum(x[1], k);
-      }
+      asm volatile("s_nop 1");   // (no MFMA between the exp2 and its use here)
+      sp_sum(x[1], k);
+      if (k & 1) sp_pack(x[1], k);
     }
     asm volatile("s_nop 7" ::: "memory");
     SB();
