@@ -129,7 +129,7 @@ def test_block_mean_of_a_slice_of_a_fused_projection(ops):
 # ---- select_blocks ---------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Bk,H,Hk,nq,nk,keep,lens", [(1, 1, 1, 1, 1, 1, 1, None), (1, 1, 2, 1, 3, 17, 5, None), (2, 2, 4, 2, 9, 65, 16, [4100, 130]), (2, 1, 3, 3, 5, 64, 64, None),
                                                        (1, 1, 1, 1, 70, 300, 37, None), (1, 1, 2, 2, 2, 30, 50, [0]), (2, 2, 1, 1, 4, 200, 1, [12800, 1]), (1, 1, 1, 1, 2, 1500, 600, None),
-                                                       (1, 1, 1, 1, 2, 5000, 700, [319999])])
+                                                       (1, 1, 1, 1, 2, 5000, 700, [319999]), (1, 1, 2, 1, 3, 20000, 900, None), (1, 1, 1, 1, 70, 2049, 2048, None)])
 def test_select_blocks(ops, B, Bk, H, Hk, nq, nk, keep, lens):
     g = gen(nk + keep)
     qm = torch.randn(B, H, nq, 128, generator=g, device="cuda")

@@ -470,6 +470,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
       if (PARTS) {
+        if ((int64_t)qb * Q_BLOCK + row >= p.Lq) continue;   // (one query of a block: its row alone, not 64 KB of sums)
         float* o = p.part + ((int64_t)wg * Q_BLOCK + row) * 128 + 4 * ge;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<float4*>(o + 16 * dt) = make_float4(x[c].accO[dt][qt][0], x[c].accO[dt][qt][1], x[c].accO[dt][qt][2], x[c].accO[dt][qt][3]);
@@ -493,31 +494,31 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     }
 }
 
-// o = sum of the parts' sums, each scaled from its own reference to the largest, over the row sums likewise: 8 rows x 32 lanes of four columns
+// o = sum of the parts' sums, each scaled from its own reference to the largest, over the row sums likewise: one wave per row, two columns a lane
 __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs) {
-  const int id = blockIdx.x, row = blockIdx.y * 8 + (threadIdx.x >> 5), c = threadIdx.x & 31;
+  const int id = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
   const int64_t r = (int64_t)qb * Q_BLOCK + row;
   if (r >= p.Lq) return;
-  const float* o = p.part + ((int64_t)id * p.parts * Q_BLOCK + row) * 128 + 4 * c;
   const float2* st = reinterpret_cast<const float2*>(p.part + (int64_t)wgs * Q_BLOCK * 128) + (int64_t)id * p.parts * Q_BLOCK + row;
-  float top = -INFINITY;
-  for (int k = 0; k < p.parts; ++k) top = fmaxf(top, st[k * Q_BLOCK].x);
-  float s[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  if (top != -INFINITY) {
-    for (int k = 0; k < p.parts; ++k) {
-      const float2 ml = st[k * Q_BLOCK];
-      const float4 v = *reinterpret_cast<const float4*>(o + (int64_t)k * Q_BLOCK * 128);
-      const float a = __builtin_amdgcn_exp2f(ml.x - top);
-      l += ml.y * a;
-      s[0] += v.x * a; s[1] += v.y * a; s[2] += v.z * a; s[3] += v.w * a;
-    }
+  const float2 ml = lane < p.parts ? st[lane * Q_BLOCK] : make_float2(-INFINITY, 0.f);   // (at most 32 parts)
+  const float top = wave_max(ml.x);
+  const float a = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+  const float l = wave_sum(ml.y * a);
+  const float* o = p.part + ((int64_t)id * p.parts * Q_BLOCK + row) * 128 + 2 * lane;
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < p.parts; ++k) {
+    const float2 v = *reinterpret_cast<const float2*>(o + (int64_t)k * Q_BLOCK * 128);
+    const float ak = __shfl(a, k, 64);
+    s0 += v.x * ak;
+    s1 += v.y * ak;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 4 * c) = make_uint2(cvt_pk(s[0] * inv, s[1] * inv), cvt_pk(s[2] * inv, s[3] * inv));
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // a row without keys: zeros
+  *reinterpret_cast<uint32_t*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 2 * lane) = cvt_pk(s0 * inv, s1 * inv);
 }
 
-// how many workgroups share a list: enough for two on every CU, a share no shorter than SPARSE_MIN_SHARE blocks
+// how many workgroups share a list: enough for two on every CU, a share no shorter than two blocks
 int sparse_parts(int64_t lists, int keep) {
   int64_t n = 512 / lists;
   if (n > keep / 2) n = keep / 2;
@@ -560,7 +561,7 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   } else {
     hipLaunchKernelGGL(attn_sparse_kernel<true>, dim3((unsigned)(lists * parts)), dim3(128), 0, st, a);
     const int64_t rows = Lq < Q_BLOCK ? Lq : Q_BLOCK;
-    hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)lists, (unsigned)((rows + 7) / 8)), dim3(256), 0, st, a, (int)(lists * parts));
+    hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)lists, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (int)(lists * parts));
   }
   WAN_LAUNCH_CHECK();
   return 0;

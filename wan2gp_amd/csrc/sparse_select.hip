@@ -13,43 +13,50 @@ namespace {
 constexpr int KEY_BLOCK = 64;
 
 // ---- block means -----------------------------------------------------------------------------------------------------------------------
-// One workgroup per (block of tokens, 128-column head group, batch): a thread owns 8 columns (16-byte loads) and every fourth row.
+// One workgroup per (block of tokens, two heads, batch): a thread owns 8 columns (16-byte loads) and every eighth row, eight loads in flight.  Bound by
+// the rows' bytes: 75,600 rows of 40 heads in 145 us, 5.3 TB/s.
 __global__ __launch_bounds__(256) void block_mean_kernel(const bf16_t* __restrict__ x, int64_t row_stride, int64_t batch_stride, const int* __restrict__ lens,
                                                         float* __restrict__ out, int64_t L, int H, int block, int nblk) {
-  __shared__ double part[3][64][8];
+  __shared__ double part[8][32][9];   // (a pitch of 9: the sums below read along the second index)
   const int n = blockIdx.x, b = blockIdx.z;
-  const int col8 = blockIdx.y * 64 + (threadIdx.x & 63), rg = threadIdx.x >> 6;   // four heads of 16 chunks per workgroup
+  const int c = threadIdx.x & 31, rg = threadIdx.x >> 5;
+  const int col8 = blockIdx.y * 32 + c;
   int64_t end = L;
   if (lens != nullptr) end = min(max((int64_t)lens[b], (int64_t)0), L);
   const int64_t r0 = (int64_t)n * block;
   const int rows = (int)min((int64_t)block, max(end - r0, (int64_t)0));
   double s[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
-  const bool live = col8 < H * 16;
-  if (live) {
+  if (col8 < H * 16) {
     const bf16_t* p = x + (int64_t)b * batch_stride + r0 * row_stride + (int64_t)col8 * 8;
-#pragma unroll 8
-    for (int r = rg; r < rows; r += 4) {
+    int r = rg;
+    for (; r + 56 < rows; r += 64) {
+      uint4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const uint4*>(p + (int64_t)(r + 8 * u) * row_stride);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float f[8];
+        unpack8(v[u], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += (double)f[j];
+      }
+    }
+    for (; r < rows; r += 8) {
       float f[8];
       unpack8(*reinterpret_cast<const uint4*>(p + (int64_t)r * row_stride), f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += (double)f[j];
     }
   }
-  if (rg > 0) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[rg - 1][threadIdx.x & 63][j] = s[j];
-  }
+  for (int j = 0; j < 8; ++j) part[rg][c][j] = s[j];
   __syncthreads();
-  if (rg == 0 && live) {
-    float m[8];
+  const int col = threadIdx.x, h = blockIdx.y * 2 + (col >> 7);   // a column a thread
+  if (h < H) {
+    double t = 0.;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double t = s[j] + part[0][threadIdx.x][j] + part[1][threadIdx.x][j] + part[2][threadIdx.x][j];
-      m[j] = rows > 0 ? (float)(t / (double)rows) : 0.f;
-    }
-    float* o = out + (((int64_t)b * H + (col8 >> 4)) * nblk + n) * 128 + (col8 & 15) * 8;
-    *reinterpret_cast<float4*>(o) = make_float4(m[0], m[1], m[2], m[3]);
-    *reinterpret_cast<float4*>(o + 4) = make_float4(m[4], m[5], m[6], m[7]);
+    for (int k = 0; k < 8; ++k) t += part[k][col >> 3][col & 7];
+    out[(((int64_t)b * H + h) * nblk + n) * 128 + (col & 127)] = rows > 0 ? (float)(t / (double)rows) : 0.f;
   }
 }
 
@@ -63,50 +70,134 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
-// keys[row][j] for 64 query blocks x 64 key blocks of one (batch, head)
+// keys[row][j], on v_mfma_f64_16x16x4_f64: lane (n, g) supplies A[n][g] (query block n) and B[g][n] (key block n) of a step; register i holds D[4 i + g][n].  A
+// sum's order is free, so step 4 s + e takes column 16 s + 4 g + e: a load of four floats a lane is 64 consecutive bytes of each row (32 consecutive floats a
+// lane read every line of the L2 four times: 223 us).  One wave per 16 query blocks x KEY_TILES tiles of
+// 16 key blocks; the query block's 32 doubles stay in registers, and the four waves of a workgroup read the same keys.  Bound by the fp64 matrix rate (a step 64
+// cycles) and the conversions in front of it: 40 heads x 591 x 1,182 in 173 us, 41 TFLOP/s and 223 MB of scores written.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr int KEY_TILES = 8;
 __global__ __launch_bounds__(256) void block_score_kernel(const float* __restrict__ qm, const float* __restrict__ km, uint64_t* __restrict__ keys, int H, int Hk,
                                                          int Bk, int nq, int nk) {
-  __shared__ float qs[64][33], ks[64][33];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int bh = blockIdx.z, b = bh / H, h = bh - b * H;
-  const float* qp = qm + (int64_t)bh * nq * 128;
-  const float* kp = km + ((int64_t)(b % Bk) * Hk + h / (H / Hk)) * nk * 128;
-  const int q0 = blockIdx.y * 64, k0 = blockIdx.x * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  double acc[4][4] = {};
-  for (int d0 = 0; d0 < 128; d0 += 32) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      const int r = i >> 5, c = i & 31;
-      qs[r][c] = q0 + r < nq ? qp[(int64_t)(q0 + r) * 128 + d0 + c] : 0.f;
-      ks[r][c] = k0 + r < nk ? kp[(int64_t)(k0 + r) * 128 + d0 + c] : 0.f;
-    }
-    __syncthreads();
-    for (int c = 0; c < 32; ++c) {
-      double a[4], w[4];
+  const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 16, k0 = blockIdx.x * (16 * KEY_TILES);
+  if (q0 >= nq) return;
+  const float* qp = qm + ((int64_t)bh * nq + min(q0 + n, nq - 1)) * 128 + 4 * g;
+  const float* kp = km + ((int64_t)(b % Bk) * Hk + h / (H / Hk)) * nk * 128 + 4 * g;
+  double a[32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { a[i] = (double)qs[ty + 16 * i][c]; w[i] = (double)ks[tx + 16 * i][c]; }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_fma(a[i], w[j], acc[i][j]);
-    }
+  for (int s = 0; s < 32; s += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(qp + 4 * s);
+    a[s] = v.x; a[s + 1] = v.y; a[s + 2] = v.z; a[s + 3] = v.w;
   }
+  // two tiles at a time: two independent chains of products, and twice the loads in flight
+  for (int t = 0; t < KEY_TILES && k0 + 16 * t < nk; t += 2) {
+    float4 v[2][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int u = 0; u < 2; ++u) {
+      const float* r = kp + (int64_t)min(k0 + 16 * (t + u) + n, nk - 1) * 128;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int q = q0 + ty + 16 * i, k = k0 + tx + 16 * j;
-      if (q < nq && k < nk) keys[((int64_t)bh * nq + q) * nk + k] = order_key(acc[i][j]);
+      for (int s = 0; s < 8; ++s) v[u][s] = *reinterpret_cast<const float4*>(r + 16 * s);
     }
+    f64x4 acc[2] = {{0., 0., 0., 0.}, {0., 0., 0., 0.}};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float f[2][4] = {{v[0][s].x, v[0][s].y, v[0][s].z, v[0][s].w}, {v[1][s].x, v[1][s].y, v[1][s].z, v[1][s].w}};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * s + e], (double)f[0][e], acc[0], 0, 0, 0);
+        acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * s + e], (double)f[1][e], acc[1], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int q = q0 + 4 * i + g, k = k0 + 16 * (t + u) + n;
+        if (q < nq && k < nk) keys[((int64_t)bh * nq + q) * nk + k] = order_key(acc[u][i]);
+      }
+  }
 }
 
 // ---- the `keep` largest of a row ---------------------------------------------------------------------------------------------------------
-// One workgroup per row, the row's keys in LDS: the keep-th largest key bit by bit from the top, then one pass that emits what is above it and the
-// first of what equals it, in ascending order.
-__global__ __launch_bounds__(256) void block_select_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
+// Both kernels find the keep-th largest key bit by bit from the top (t: the largest value that at least `want` keys reach; they stop as soon as exactly that
+// many do), then emit what is above it and the first of what equals it, in ascending order.  A key 0 is none.
+
+// One wave per row, N keys a lane in registers, first over the keys' upper halves -- 20 of the mantissa's bits decide nearly every row.
+// Bound by the scores' bytes and the ballots: 23,640 rows of 1,182 in 60 us, 3.7 TB/s.  The whole choice took 236 us so and 390 us with the
+// search by a workgroup below; 33 against 59 us at 128 x 256, 609 against 937 us at 1,024 x 2,048.
+template <int N>
+__global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
+                                                               int* __restrict__ count, int H, int Bk, int nq, int nk, int keep, int64_t rows) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const int b = (int)(r / ((int64_t)H * nq));
+  int n = nk;
+  if (k_lens != nullptr) n = min(nk, max(0, (int)(((int64_t)k_lens[b % Bk] + KEY_BLOCK - 1) / KEY_BLOCK)));
+  int* idx = index + r * keep;
+  const int want = min(keep, n);
+  if (lane == 0) count[r] = want;
+  for (int i = want + lane; i < keep; i += 64) idx[i] = -1;
+  if (want == n) {
+    for (int i = lane; i < n; i += 64) idx[i] = i;
+    return;
+  }
+  uint32_t hi[N], lo[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = j * 64 + lane;
+    const uint64_t k = i < n ? keys[r * nk + i] : 0ull;
+    hi[j] = (uint32_t)(k >> 32);
+    lo[j] = (uint32_t)k;
+  }
+  uint32_t th = 0, tl = 0;
+  int ge = n;
+  for (int bit = 31; bit >= 0 && ge != want; --bit) {
+    const uint32_t c = th | (1u << bit);
+    int m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m += __popcll(__ballot(hi[j] >= c));
+    if (m >= want) { th = c; ge = m; }
+  }
+  if (ge != want) {
+    for (int bit = 31; bit >= 0 && ge != want; --bit) {
+      const uint32_t c = tl | (1u << bit);
+      int m = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) m += __popcll(__ballot(hi[j] > th || (hi[j] == th && lo[j] >= c)));
+      if (m >= want) { tl = c; ge = m; }
+    }
+  }
+  int room = n;          // how many of the keys that equal t are taken
+  if (ge != want) {
+    int above = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) above += __popcll(__ballot(hi[j] > th || (hi[j] == th && lo[j] > tl)));
+    room = want - above;
+  }
+  int out = 0;
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const bool eq = hi[j] == th && lo[j] == tl;
+    const uint64_t eqs = __ballot(eq);
+    const bool take = hi[j] > th || (hi[j] == th && lo[j] > tl) || (eq && __popcll(eqs & below) < room);
+    const uint64_t tk = __ballot(take);
+    if (take) idx[out + __popcll(tk & below)] = j * 64 + lane;
+    out += __popcll(tk);
+    room -= min(room, (int)__popcll(eqs));
+  }
+}
+
+// More than 2,048 blocks: one workgroup per row, the row's keys in LDS.  16 waves where the LDS has room for two rows or fewer (128 x 20,000 of 40 heads: 2.49 ms,
+// with 4 waves 4.35), else 4, more workgroups side by side (512 x 4,096: 1.31 ms, with 16 waves 1.67).
+template <int WG_WAVES>
+__global__ __launch_bounds__(64 * WG_WAVES) void block_select_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
                                                           int* __restrict__ count, int H, int Bk, int nq, int nk, int keep) {
   extern __shared__ uint64_t row[];
-  __shared__ int wsum[2][4];
+  __shared__ int wsum[2][WG_WAVES];
   const int64_t r = blockIdx.x;
   const int b = (int)(r / ((int64_t)H * nq));
   int n = nk;
@@ -115,35 +206,38 @@ __global__ __launch_bounds__(256) void block_select_kernel(const uint64_t* __res
   int* idx = index + r * keep;
   const int want = min(keep, n);
   if (tid == 0) count[r] = want;
-  for (int i = want + tid; i < keep; i += 256) idx[i] = -1;
+  for (int i = want + tid; i < keep; i += 64 * WG_WAVES) idx[i] = -1;
   if (want == n) {
-    for (int i = tid; i < n; i += 256) idx[i] = i;
+    for (int i = tid; i < n; i += 64 * WG_WAVES) idx[i] = i;
     return;
   }
-  for (int i = tid; i < n; i += 256) row[i] = keys[r * nk + i];
+  for (int i = tid; i < n; i += 64 * WG_WAVES) row[i] = keys[r * nk + i];
   __syncthreads();
-  uint64_t t = 0;      // the largest value that at least `want` keys reach
-  int ge = n;          // how many reach it
+  uint64_t t = 0;
+  int ge = n;
   for (int bit = 63; bit >= 0 && ge != want; --bit) {
     const uint64_t c = t | (1ull << bit);
     int m = 0;
-    for (int i = tid; i < n; i += 256) m += row[i] >= c;
+    for (int i = tid; i < n; i += 64 * WG_WAVES) m += row[i] >= c;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
     if (lane == 0) wsum[bit & 1][wave] = m;
     __syncthreads();
-    m = wsum[bit & 1][0] + wsum[bit & 1][1] + wsum[bit & 1][2] + wsum[bit & 1][3];
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < WG_WAVES; ++w) m += wsum[bit & 1][w];
     if (m >= want) { t = c; ge = m; }
   }
-  // more than `want` keys reach t only if the smallest of them equal t: the first of those are taken
   int above = 0;
-  for (int i = tid; i < n; i += 256) above += row[i] > t;
+  for (int i = tid; i < n; i += 64 * WG_WAVES) above += row[i] > t;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) above += __shfl_xor(above, o, 64);
   __syncthreads();
   if (lane == 0) wsum[0][wave] = above;
   __syncthreads();
-  above = wsum[0][0] + wsum[0][1] + wsum[0][2] + wsum[0][3];
+  above = 0;
+#pragma unroll
+  for (int w = 0; w < WG_WAVES; ++w) above += wsum[0][w];
   if (wave != 0) return;
   int room = ge == want ? n : want - above, out = 0;   // room: how many of the keys that equal t are still taken
   for (int i0 = 0; i0 < n; i0 += 64) {
@@ -167,8 +261,8 @@ extern "C" int wan_block_mean(const wan_bf16* x, int64_t row_stride, int64_t bat
   WAN_REQUIRE(row_stride % 8 == 0 && batch_stride % 8 == 0 && row_stride >= (int64_t)H * 128, "wan_block_mean: strides must be multiples of 8 elements, a row's at least H * 128");
   WAN_REQUIRE((((uintptr_t)x | (uintptr_t)out) & 15) == 0, "wan_block_mean: pointers must be 16-byte aligned");
   const int64_t nblk = (L + block - 1) / block;
-  WAN_REQUIRE(nblk < ((int64_t)1 << 31) && B < 65536 && H <= 4 * 65535, "wan_block_mean: grid too large");
-  hipLaunchKernelGGL(block_mean_kernel, dim3((unsigned)nblk, (unsigned)((H * 16 + 63) / 64), (unsigned)B), dim3(256), 0, as_stream(stream), x, row_stride, batch_stride, lens, out,
+  WAN_REQUIRE(nblk < ((int64_t)1 << 31) && B < 65536 && H <= 2 * 65535, "wan_block_mean: grid too large");
+  hipLaunchKernelGGL(block_mean_kernel, dim3((unsigned)nblk, (unsigned)((H + 1) / 2), (unsigned)B), dim3(256), 0, as_stream(stream), x, row_stride, batch_stride, lens, out,
                      L, H, block, (int)nblk);
   WAN_LAUNCH_CHECK();
   return 0;
@@ -192,9 +286,19 @@ extern "C" int wan_select_blocks(const float* q_mean, const float* k_mean, const
   WAN_REQUIRE((((uintptr_t)q_mean | (uintptr_t)k_mean) & 15) == 0, "wan_select_blocks: the means must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
   uint64_t* keys = reinterpret_cast<uint64_t*>(scratch);
-  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 63) / 64), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean, keys, H, Hk, Bk, (int)nq, (int)nk);
+  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 16 * KEY_TILES - 1) / (16 * KEY_TILES)), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean,
+                     keys, H, Hk, Bk, (int)nq, (int)nk);
   WAN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(block_select_kernel, dim3((unsigned)(B * H * nq)), dim3(256), (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+  const int64_t rows = (int64_t)B * H * nq;
+  const dim3 grid((unsigned)((rows + 3) / 4)), wg(256);
+#define SELECT(N) hipLaunchKernelGGL(block_select_wave_kernel<N>, grid, wg, 0, st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep, rows)
+  if (nk <= 256) SELECT(4);
+  else if (nk <= 640) SELECT(10);
+  else if (nk <= 1216) SELECT(19);
+  else if (nk <= 2048) SELECT(32);
+  else if (nk <= 6800) hipLaunchKernelGGL(block_select_kernel<4>, dim3((unsigned)rows), wg, (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+  else hipLaunchKernelGGL(block_select_kernel<16>, dim3((unsigned)rows), dim3(1024), (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+#undef SELECT
   WAN_LAUNCH_CHECK();
   return 0;
 }
