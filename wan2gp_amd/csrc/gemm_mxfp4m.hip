@@ -3,6 +3,9 @@
 // Half a byte per element makes a k-stage of 256 values exactly gemm256m's 128-byte rows: unit images (256 rows x 128 B), swizzle, ring of five 32-KB
 // units, fragment reads and register-direct stores carry over, and a k-step of 128 is 64 MFMAs of 16 cycles (v_mfma_scale_f32_16x16x128_f8f6f4 on
 // two fp4 operands) where gemm256m's of 32 is 64 MFMAs of 16 cycles -- four times the FLOP on the same bytes and issue slots.  What differs:
+//   * one workgroup a CU takes one tile after the other, and the streams of units run on into the next tile: its first stages land and this tile's stores
+//     drain while the other of the two is worked on (a workgroup a tile: 32,760 x 8,960 x 1,536 297 us, so 255; with the GELU 356 and 310).  The tile
+//     loop has one stage body with its ring slots in scalar registers.
 //   * both operands' image rows are (slab, t, n) = row slab * 128 + 8 n + t: a lane's eight scales of an operand and k-step are then 8 consecutive
 //     bytes of mxfp4_ops.hip's scale tiles, and all of a stage's one 16-byte load (dword 2 ks + (t >> 2), byte t & 3: the instruction picks the
 //     byte).  y tile a, register i of lane (n, g) is row 8 (4 g + i) + a.
@@ -12,6 +15,10 @@
 //     80 MFMAs (1,280 cycles) by then.
 //   * K need not be a multiple of 256: what a row's last stage reads past the row is the next row's codes (the buffer's end reads as zeros), and the
 //     scale bytes there are 0 on both sides -- (6 * 2^-127)^2 is 0 in fp32.
+//   * stores are non-temporal: 256 tiles are 32 MB, more than the L2 keeps for whoever reads them (with ordinary stores 268 us for 255 above).
+// Bound by the card's power where K is long: 75,600 x 5,120 x 13,824 with the gated residual in 2.34 ms, 4.6 PFLOP/s, 67 % of the cycles on the matrix pipe
+// at 1.4 GHz; the same MFMAs with no memory access between them would take 1.75 ms.  Where K is short, by the epilogue: at K = 1,536 the GELU's
+// 52 VALU cycles an element are as much as the products' (310 us, 2.9 PFLOP/s).
 #include "mxfp4.h"
 
 namespace {
@@ -50,216 +57,272 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   const int wy = wave >> 1, wx = wave & 1;
   const int l15 = lane & 15, lg = lane >> 4;
 
-  // XCD-contiguous ids, then groups of `group` tile rows walked column by column: the tiles that run at a time share few panels
-  const int wg = xcd_remap(blockIdx.x, tiles_y * tiles_x);
+  // A workgroup takes every step-th tile of its XCD's contiguous range of ids; ids run through groups of `group` tile rows column by column, so that the
+  // tiles that an XCD works on at a time share few panels
+  const int tiles = tiles_y * tiles_x;
+  const int xcd = blockIdx.x & 7, qt = tiles >> 3, rt = tiles & 7;
+  const int first = xcd < rt ? xcd * (qt + 1) : rt * (qt + 1) + (xcd - rt) * qt, end = first + qt + (xcd < rt ? 1 : 0);
+  const int step = ((int)gridDim.x >> 3) + (xcd < ((int)gridDim.x & 7) ? 1 : 0);
+  int tile = first + (blockIdx.x >> 3);
   const int per_group = group * tiles_x;
-  const int gidx = wg / per_group;
-  const int first_y = gidx * group;
-  const int gsz = min(tiles_y - first_y, group);
-  const int in_g = wg - gidx * per_group;
-  const int64_t y0 = (int64_t)(first_y + in_g % gsz) * MXM_BM;
-  const int64_t x0 = (int64_t)(in_g / gsz) * MXM_BN;
+  struct Tile {
+    int y, x;   // in units of 256
+  };
+  auto decode = [&](int t) -> Tile {
+    const int gi = t / per_group, fy = gi * group, gsz = min(tiles_y - fy, group), in_g = t - gi * per_group, x = in_g / gsz;
+    return {__builtin_amdgcn_readfirstlane(fy + in_g - x * gsz), __builtin_amdgcn_readfirstlane(x)};
+  };
 
-  // DMA plan: piece i of wave w fills the 16-byte slots q = i * 256 + w * 64 + lane; image row q >> 3, physical chunk q & 7 = logical ^ ((row >> 1) & 7)
+  // DMA plan: piece i of wave w fills the 16-byte slots q = i * 256 + w * 64 + lane; image row q >> 3, physical chunk q & 7 = logical ^ ((row >> 1) & 7).
+  // Rows past the matrix lie past the descriptor's end: zeros, never stored
   const int pitch = p.K / 2;
-  uint32_t yofs[8], xofs[8];
+  uint32_t ofs[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int q = i * 256 + tid;
     const int row = q >> 3, lch = (q & 7) ^ ((row >> 1) & 7);
     const int r = (row >> 7) * 128 + 8 * (row & 15) + ((row >> 4) & 7);
-    yofs[i] = (uint32_t)(min(y0 + r, p.M - 1) - y0) * (uint32_t)pitch + lch * 16;   // past the matrix: its last row again, never stored
-    xofs[i] = (uint32_t)(min(x0 + r, p.N - 1) - x0) * (uint32_t)pitch + lch * 16;
+    ofs[i] = (uint32_t)r * (uint32_t)pitch + lch * 16;
+    asm volatile("" : "+v"(ofs[i]));
   }
-  const char* ybase = reinterpret_cast<const char*>(p.A) + y0 * pitch;
-  const char* xbase = reinterpret_cast<const char*>(p.W) + x0 * pitch;
-  uint32_t yrec = (uint32_t)min((p.M - y0) * pitch, (int64_t)0xffffff00);
-  uint32_t xrec = (uint32_t)min((p.N - x0) * pitch, (int64_t)0xffffff00);
-  const uint32_t smem_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  const uint32_t smem_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 1024;
   const int nk = p.kt;
-  int ky = 0, kx = 0;  // the stages the two streams point at; they stop at the last one
-  auto y_piece = [&](int slot, int i) { mx_dma16(yofs[i], mx_rsrc(ybase, yrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
-  auto x_piece = [&](int slot, int i) { mx_dma16(xofs[i], mx_rsrc(xbase, xrec), smem_lds + slot * MXM_UNIT + (i * 256 + wave * 64) * 16); };
-  auto y_advance = [&]() { const int s = ky + 1 < nk ? MXM_ROW : 0; ybase += s; yrec -= s; ky += s ? 1 : 0; };
-  auto x_advance = [&]() { const int s = kx + 1 < nk ? MXM_ROW : 0; xbase += s; xrec -= s; kx += s ? 1 : 0; };
+  // The streams of Y units, X units and scales run ahead of the products, through the stages of one tile after the other: the next tile's first stages are
+  // on their way while this one's epilogue runs.  Past the last tile they stay at its last stage.
+  struct Stream {
+    const char* base;
+    uint32_t rec;
+    int tile, k;
+  };
+  auto enter = [&](Stream& st, int t, bool is_y) {
+    const Tile at = decode(t);
+    const int64_t r0 = (int64_t)(is_y ? at.y : at.x) * 256, rows = (is_y ? p.M : p.N) - r0;
+    st.base = reinterpret_cast<const char*>(is_y ? p.A : p.W) + r0 * pitch;
+    st.rec = (uint32_t)min(rows * pitch, (int64_t)0xffffff00);
+    st.tile = t;
+    st.k = 0;
+  };
+  auto advance = [&](Stream& st, bool is_y) {
+    if (st.k + 1 < nk) {
+      st.base += MXM_ROW;
+      st.rec -= MXM_ROW;
+      ++st.k;
+    } else if (st.tile + step < end) {
+      enter(st, st.tile + step, is_y);
+    }
+  };
+  auto piece = [&](const Stream& st, uint32_t slot, int i) { mx_dma16(ofs[i], mx_rsrc(st.base, st.rec), smem_lds + slot + i * 4096); };
+  // a lane's scales: 16 bytes a stage of each operand's 128-row panel
+  struct Scales {
+    const char *y, *x;
+    int tile, k;
+  };
+  auto enter_scales = [&](Scales& st, int t) {
+    const Tile at = decode(t);
+    st.y = reinterpret_cast<const char*>(p.As) + min((int64_t)at.y * 2 + wy, (p.M - 1) >> 7) * nk * 1024;
+    st.x = reinterpret_cast<const char*>(p.Ws) + min((int64_t)at.x * 2 + wx, (p.N - 1) >> 7) * nk * 1024;
+    st.tile = t;
+    st.k = 0;
+  };
+  auto advance_scales = [&](Scales& st) {
+    if (st.k + 1 < nk) {
+      st.y += 1024;
+      st.x += 1024;
+      ++st.k;
+    } else if (st.tile + step < end) {
+      enter_scales(st, st.tile + step);
+    }
+  };
+  auto scale_of = [&](const char* q) { return *reinterpret_cast<const mx_u4*>(q + lane * 16); };
 
-  // the lane's scales: 16 bytes a stage of each operand's 128-row panel
-  const mx_u4* ysc = reinterpret_cast<const mx_u4*>(p.As + min((y0 >> 7) + wy, (p.M - 1) >> 7) * nk * 1024) + lg * 16 + l15;
-  const mx_u4* xsc = reinterpret_cast<const mx_u4*>(p.Ws + min((x0 >> 7) + wx, (p.N - 1) >> 7) * nk * 1024) + lg * 16 + l15;
-
-  // fragment addresses: one base register per (operand, k-step, 64-KB window) and immediates (gemm256m.hip)
+  // fragment addresses: one base per (operand, k-step), the tiles 2 KB apart
   const int sw = (l15 >> 1) & 7;
-  uint32_t ybw[2][3], xbw[2][3];
+  uint32_t ybw[2], xbw[2];
 #pragma unroll
-  for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      ybw[ks][w] = (uint32_t)((((wy * 128 + l15) * 128 + ((lg ^ sw) << 4)) ^ (ks << 6)) + w * 65536);
-      xbw[ks][w] = (uint32_t)((((wx * 128 + l15) * 128 + ((lg ^ sw) << 4)) ^ (ks << 6)) + w * 65536);
-      asm volatile("" : "+v"(ybw[ks][w]), "+v"(xbw[ks][w]));
-    }
-  auto load_frag = [&](MxmFrags& f, int sy, int sx, int ks, int r) {
-    if (r < 8) {
-      const int u = sy * MXM_UNIT + r * 2048;
-      f.y[r] = *(mxm_lds_u4*)(lds + ybw[ks][u >> 16] + (u & 0xffff));
-    } else {
-      const int u = sx * MXM_UNIT + (r - 8) * 2048;
-      f.x[r - 8] = *(mxm_lds_u4*)(lds + xbw[ks][u >> 16] + (u & 0xffff));
-    }
+  for (int ks = 0; ks < 2; ++ks) {
+    ybw[ks] = (uint32_t)(((wy * 128 + l15) * 128 + ((lg ^ sw) << 4)) ^ (ks << 6));
+    xbw[ks] = (uint32_t)(((wx * 128 + l15) * 128 + ((lg ^ sw) << 4)) ^ (ks << 6));
+  }
+  auto load_frag = [&](MxmFrags& f, uint32_t ya, uint32_t xa, int r) {
+    if (r < 8) f.y[r] = *(mxm_lds_u4*)(lds + ya + r * 2048);
+    else f.x[r - 8] = *(mxm_lds_u4*)(lds + xa + (r - 8) * 2048);
   };
   // the order of a k-step's 16 fragment reads: y 1 .. 7, x 1 .. 7, x 0, y 0 -- what its first MFMA needs comes last, so that ONE wait covers all
   auto ord = [](int i) constexpr { return i < 7 ? 1 + i : i < 14 ? 2 + i : i == 14 ? 8 : 0; };
+  auto next_slot = [](uint32_t s) -> uint32_t { return s + MXM_UNIT == MXM_NU * MXM_UNIT ? 0u : s + MXM_UNIT; };
 
-  mx_u4 sy = ysc[0], sx = xsc[0];
+  Stream ys, xs;
+  Scales ss;
+  enter(ys, tile, true);
+  enter(xs, tile, false);
+  enter_scales(ss, tile);
+  mx_u4 sy = scale_of(ss.y), sx = scale_of(ss.x);
   asm volatile("" : "+v"(sy), "+v"(sx));
+  advance_scales(ss);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y_piece(0, i);
-  y_advance();
+  for (int u = 0; u < 5; ++u) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x_piece(1, i);
-  x_advance();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y_piece(2, i);
-  y_advance();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x_piece(3, i);
-  x_advance();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y_piece(4, i);
-  y_advance();
-  f32x4 acc[8][8];
-#pragma unroll
-  for (int a = 0; a < 8; ++a)
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[a][b][r] = 0.f;
-      asm volatile("" : "+a"(acc[a][b]));
-    }
+    for (int i = 0; i < 8; ++i) piece((u & 1) ? xs : ys, u * MXM_UNIT, i);
+    if (u & 1) advance(xs, false);
+    else advance(ys, true);
+  }
   asm volatile("s_waitcnt vmcnt(24)" ::: "memory");  // stage 0 landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   MxmFrags f0, f1;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) load_frag(f0, 0, 1, 0, ord(r));
-  // Stage S = 5 i + J: Y in slot 2J % 5, X in (2J + 1) % 5.
-  //   k-step 0 (f0): stage S + 1's scales behind MFMA 0, k-step 1's fragments behind MFMA 1, 3, .., 31
-  //   k-step 1 (f1): MFMAs 0 .. 15 bare
-  //   P_S: everything landed, stage S fully read + barrier
-  //   MFMAs 16 .. 63: X_{S+2} -> slot of Y_S behind 16, 19, .., 37, Y_{S+3} -> slot of X_S behind 40, 43, .., 61; stage S + 1's first fragments
-  //                   in the other gaps up to MFMA 39
-  mx_u4 ny, nx;
-#define MXM_STAGE(J)                                                                                                             \
-  if (__builtin_expect(kt + (J) < nk, 1)) {                                                                                      \
-    constexpr int J_ = (J);                                                                                                      \
-    constexpr int SY = (2 * J_) % 5, SX = (2 * J_ + 1) % 5, NY = (2 * J_ + 2) % 5, NX = (2 * J_ + 3) % 5;                         \
-    mxm_run<0, 0, 64>(acc, f0, sy, sx, [&](int m) __attribute__((always_inline)) {                                               \
-      if (m == 0) {                                                                                                              \
-        const int64_t at = (int64_t)min(kt + J_ + 1, nk - 1) * 64;                                                               \
-        ny = ysc[at];                                                                                                            \
-        nx = xsc[at];                                                                                                            \
-      }                                                                                                                          \
-      if ((m & 1) == 1 && m < 32) load_frag(f1, SY, SX, 1, ord(m >> 1));                                                         \
-    });                                                                                                                          \
-    mxm_run<1, 0, 16>(acc, f1, sy, sx, [](int) {});                                                                              \
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                                                                  \
-    __builtin_amdgcn_s_barrier();                                                                                                \
-    asm volatile("" : "+v"(ny), "+v"(nx)::"memory");                                                                             \
-    mxm_run<1, 16, 64>(acc, f1, sy, sx, [&](int m) __attribute__((always_inline)) {                                              \
-      const int q = (m - 16) / 3, r = (m - 16) % 3;                                                                              \
-      if (r == 0 && q < 8) x_piece(SY, q);                                                                                       \
-      if (r == 0 && q >= 8) y_piece(SX, q - 8);                                                                                  \
-      if (r != 0 && q < 8) load_frag(f0, NY, NX, 0, ord(2 * q + r - 1));                                                         \
-    });                                                                                                                          \
-    x_advance();                                                                                                                 \
-    y_advance();                                                                                                                 \
-    sy = ny;                                                                                                                     \
-    sx = nx;                                                                                                                     \
-    asm volatile("s_nop 1" : "+v"(sy), "+v"(sx)); /* a register copy in front of an MFMA that reads it: hipcc pads nothing around asm */ \
-  }
-  for (int kt = 0; kt < nk; kt += 5) {
-    MXM_STAGE(0)
-    MXM_STAGE(1)
-    MXM_STAGE(2)
-    MXM_STAGE(3)
-    MXM_STAGE(4)
-  }
-#undef MXM_STAGE
-  // trailing DMA (the LDS is released at the end); the last MFMAs -> accumulator reads
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  for (int r = 0; r < 16; ++r) load_frag(f0, ybw[0], xbw[0] + MXM_UNIT, ord(r));
+  uint32_t slot_y = 0;   // of the current stage
+  auto load_bias = [&](int64_t x) -> uint4 {   // of this lane's columns
+    const int64_t c = x + wx * 128 + 8 * l15;
+    return EPI != WAN_EPI_TRANSPOSED && p.bias != nullptr && c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.bias + c) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  Tile at = decode(tile);
+  uint4 bias = load_bias((int64_t)at.x * MXM_BN);
+  for (;;) {
+    f32x4 acc[8][8];
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        asm volatile("" : "+a"(acc[a][b]));
+      }
+    asm volatile("s_nop 1" ::: "memory");   // (in front of the first MFMA that reads them: hipcc pads nothing around asm)
+    // Stage S: Y in slot 2 S % 5, X in (2 S + 1) % 5 (S counted over the tiles).
+    //   k-step 0 (f0): stage S + 1's scales behind MFMA 0, k-step 1's fragments behind MFMA 1, 3, .., 31
+    //   k-step 1 (f1): MFMAs 0 .. 15 bare
+    //   P_S: everything landed, stage S fully read + barrier
+    //   MFMAs 16 .. 63: X_{S+2} -> slot of Y_S behind 16, 19, .., 37, Y_{S+3} -> slot of X_S behind 40, 43, .., 61; stage S + 1's first fragments
+    //                   in the other gaps up to MFMA 39
+#pragma unroll 1
+    for (int k = 0; k < nk; ++k) {
+      const uint32_t slot_x = next_slot(slot_y), next_y = next_slot(slot_x), next_x = next_slot(next_y);
+      const uint32_t y1 = ybw[1] + slot_y, x1 = xbw[1] + slot_x, yn = ybw[0] + next_y, xn = xbw[0] + next_x;
+      mx_u4 ny, nx;
+      mxm_run<0, 0, 64>(acc, f0, sy, sx, [&](int m) __attribute__((always_inline)) {
+        if (m == 0) {
+          ny = scale_of(ss.y);
+          nx = scale_of(ss.x);
+        }
+        if ((m & 1) == 1 && m < 32) load_frag(f1, y1, x1, ord(m >> 1));
+      });
+      advance_scales(ss);
+      mxm_run<1, 0, 16>(acc, f1, sy, sx, [](int) {});
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : "+v"(ny), "+v"(nx)::"memory");
+      mxm_run<1, 16, 64>(acc, f1, sy, sx, [&](int m) __attribute__((always_inline)) {
+        const int q = (m - 16) / 3, r = (m - 16) % 3;
+        if (r == 0 && q < 8) piece(xs, slot_y, q);
+        if (r == 0 && q >= 8) piece(ys, slot_x, q - 8);
+        if (r != 0 && q < 8) load_frag(f0, yn, xn, ord(2 * q + r - 1));
+      });
+      advance(xs, false);
+      advance(ys, true);
+      slot_y = __builtin_amdgcn_readfirstlane(next_y);
+      sy = ny;
+      sx = nx;
+      asm volatile("s_nop 1" : "+v"(sy), "+v"(sx)); /* a register copy in front of an MFMA that reads it: hipcc pads nothing around asm */
+    }
+    // the last MFMAs -> accumulator reads
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    const int64_t y0 = (int64_t)at.y * MXM_BM, x0 = (int64_t)at.x * MXM_BN;
+    float bcol[8];
+    unpack8(bias, bcol);
+    tile += step;
+    if (tile < end) {
+      at = decode(tile);
+      bias = load_bias((int64_t)at.x * MXM_BN);
+    }
 
-  // ---- epilogue: straight from the registers.  Rows past the matrix fall outside the descriptors' num_records; a lane's 8 columns are inside or
-  // outside as a whole (N % 8 == 0), outside: an offset past num_records --------------------------------------------------------------------
-  uint32_t lane_e;  // an opaque lane id: derived from threadIdx the epilogue's offsets are hoisted in front of the MFMA loop and spilled
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_e));
-  const uint32_t ne = lane_e & 15u, ge = lane_e >> 4;
-  const uint32_t colb = (uint32_t)(wx * 128) * 2u + ne * 16u;
-  const int64_t rows_valid = min(p.M - y0, (int64_t)MXM_BM);
-  const uint32_t onum = (uint32_t)((rows_valid - 1) * p.ldc * 2 + MXM_BN * 2);
-  const uint32_t ldo2 = (uint32_t)(p.ldc * 2);
-  const __amdgpu_buffer_rsrc_t odesc = __builtin_amdgcn_make_buffer_rsrc((void*)(p.C + y0 * p.ldc + x0), 0, (int)onum, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rdesc = __builtin_amdgcn_make_buffer_rsrc((void*)((EPI == WAN_EPI_GATE_RES ? p.R : p.C) + y0 * p.ldc + x0), 0, (int)onum, 0x00020000);
-  const uint32_t row_lane = (uint32_t)(wy * 128) + 32u * ge;
-  const bool col_in = x0 + wx * 128 + 8 * (int64_t)ne + 8 <= p.N;
-  const uint32_t lane_off = col_in ? row_lane * ldo2 + colb : 0x80000000u;
-  float bcol[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (EPI != WAN_EPI_TRANSPOSED && p.bias != nullptr && col_in) unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.bias + x0) + colb), bcol);
-  // gates: a 256-row tile touches at most two batches (rows_per_batch >= 256)
-  float gA[8], gB[8];
+    // ---- epilogue: straight from the registers.  Rows past the matrix fall outside the descriptors' num_records; a lane's 8 columns are inside or
+    // outside as a whole (N % 8 == 0), outside: an offset past num_records --------------------------------------------------------------------
+    // (its arguments are read from the kernel's again: held across the loop they take the scalar registers that the streams need)
+    typedef __attribute__((address_space(4))) const MxGemm mxm_args;
+    mxm_args* pe = (mxm_args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(pe));
+    uint32_t lane_e;  // an opaque lane id: derived from threadIdx the epilogue's offsets are hoisted in front of the MFMA loop and spilled
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_e));
+    const uint32_t ne = lane_e & 15u, ge = lane_e >> 4;
+    const uint32_t colb = (uint32_t)(wx * 128) * 2u + ne * 16u;
+    const int64_t rows_valid = min(pe->M - y0, (int64_t)MXM_BM);
+    const uint32_t onum = (uint32_t)((rows_valid - 1) * pe->ldc * 2 + MXM_BN * 2);
+    const uint32_t ldo2 = (uint32_t)(pe->ldc * 2);
+    const __amdgpu_buffer_rsrc_t odesc = __builtin_amdgcn_make_buffer_rsrc((void*)(pe->C + y0 * pe->ldc + x0), 0, (int)onum, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rdesc = __builtin_amdgcn_make_buffer_rsrc((void*)((EPI == WAN_EPI_GATE_RES ? pe->R : pe->C) + y0 * pe->ldc + x0), 0, (int)onum, 0x00020000);
+    const uint32_t row_lane = (uint32_t)(wy * 128) + 32u * ge;
+    const bool col_in = x0 + wx * 128 + 8 * (int64_t)ne + 8 <= pe->N;
+    const uint32_t lane_off = col_in ? row_lane * ldo2 + colb : 0x80000000u;
+    // gates: a 256-row tile touches at most two batches (rows_per_batch >= 256)
+    float gA[8], gB[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) gA[j] = gB[j] = 1.f;
-  uint32_t rb = 0xffffffffu;
-  auto gate_row = [&](int64_t bidx, float* gq) {
-    float mv[8], ev[8];
-    unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.mod + (int64_t)p.gate_idx * p.N + x0) + colb), mv);
-    unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p.e + (bidx * p.n_mod + p.gate_idx) * p.N + x0) + colb), ev);
+    for (int j = 0; j < 8; ++j) gA[j] = gB[j] = 1.f;
+    uint32_t rb = 0xffffffffu;
+    auto gate_row = [&](int64_t bidx, float* gq) {
+      float mv[8], ev[8];
+      unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(pe->mod + (int64_t)pe->gate_idx * pe->N + x0) + colb), mv);
+      unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(pe->e + (bidx * pe->n_mod + pe->gate_idx) * pe->N + x0) + colb), ev);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) gq[j] = mv[j] + ev[j];
-  };
-  if (EPI == WAN_EPI_GATE_RES && p.gate_idx >= 0 && col_in) {
-    const int64_t b0 = y0 / p.rows_per_batch;
-    const int64_t yb = (b0 + 1) * p.rows_per_batch;
-    gate_row(b0, gA);
-    if (yb < y0 + rows_valid) {
-      rb = (uint32_t)(yb - y0);
-      gate_row(b0 + 1, gB);
+      for (int j = 0; j < 8; ++j) gq[j] = mv[j] + ev[j];
+    };
+    if (EPI == WAN_EPI_GATE_RES && pe->gate_idx >= 0 && col_in) {
+      const int64_t b0 = y0 / pe->rows_per_batch;
+      const int64_t yb = (b0 + 1) * pe->rows_per_batch;
+      gate_row(b0, gA);
+      if (yb < y0 + rows_valid) {
+        rb = (uint32_t)(yb - y0);
+        gate_row(b0 + 1, gB);
+      }
     }
-  }
-  typedef unsigned int mxm_st4 __attribute__((__vector_size__(16)));
-  auto rload = [&](int a, int i) -> uint4 {
-    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rdesc, (int)(lane_off + (uint32_t)(8 * i + a) * ldo2), 0, 0));
-  };
-  uint4 rq[3][4] = {};   // residual rows of the next two y tiles are in flight while one is converted
-  if (EPI == WAN_EPI_GATE_RES) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { rq[0][i] = rload(0, i); rq[1][i] = rload(1, i); }
-  }
-#pragma unroll
-  for (int a = 0; a < 8; ++a) {
-    if (EPI == WAN_EPI_GATE_RES && a + 2 < 8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) rq[(a + 2) % 3][i] = rload(a + 2, i);
-    }
+    typedef unsigned int mxm_st4 __attribute__((__vector_size__(16)));
+    uint32_t ro[4];   // rows 8 i + a of the current a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t rit = (uint32_t)(8 * i + a);
-      float brow = 0.f;
-      if (EPI == WAN_EPI_TRANSPOSED && p.bias != nullptr) brow = bf2f(p.bias[min(y0 + row_lane + rit, p.M - 1)]);
-      float v[8], rv[8];
-      if (EPI == WAN_EPI_GATE_RES) unpack8(rq[a % 3][i], rv);
-      const bool second = row_lane + rit >= rb;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        float o = acc[a][t][i] + (EPI == WAN_EPI_TRANSPOSED ? brow : bcol[t]);
-        if (EPI == WAN_EPI_GELU_TANH) o = mx_gelu_tanh(o);
-        if (EPI == WAN_EPI_GATE_RES) o = __builtin_fmaf(o, second ? gB[t] : gA[t], rv[t]);
-        v[t] = o;
-      }
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(mxm_st4, pack8(v)), odesc, (int)(lane_off + rit * ldo2), 0, 0);
-      if (EPI == WAN_EPI_GELU_TANH) __builtin_amdgcn_sched_barrier(0);  // 8 GELUs' temporaries at a time
+      ro[i] = lane_off + (uint32_t)(8 * i) * ldo2;
+      asm volatile("" : "+v"(ro[i]));
     }
-    __builtin_amdgcn_sched_barrier(0);
+    auto rload = [&](int ahead, int i) -> uint4 {
+      return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rdesc, (int)(ro[i] + (uint32_t)ahead * ldo2), 0, 0));
+    };
+    uint4 rq[3][4] = {};   // residual rows of the next two y tiles are in flight while one is converted
+    if (EPI == WAN_EPI_GATE_RES) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { rq[0][i] = rload(0, i); rq[1][i] = rload(1, i); }
+    }
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) asm volatile("" : "+a"(acc[a][t]));   // (read here, not all 256 in front of the rows)
+      if (EPI == WAN_EPI_GATE_RES && a + 2 < 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rq[(a + 2) % 3][i] = rload(2, i);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t rit = (uint32_t)(8 * i + a);
+        float brow = 0.f;
+        if (EPI == WAN_EPI_TRANSPOSED && pe->bias != nullptr) brow = bf2f(pe->bias[min(y0 + row_lane + rit, pe->M - 1)]);
+        float v[8], rv[8];
+        if (EPI == WAN_EPI_GATE_RES) unpack8(rq[a % 3][i], rv);
+        const bool second = row_lane + rit >= rb;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          float o = acc[a][t][i] + (EPI == WAN_EPI_TRANSPOSED ? brow : bcol[t]);
+          if (EPI == WAN_EPI_GELU_TANH) o = mx_gelu_tanh(o);
+          if (EPI == WAN_EPI_GATE_RES) o = __builtin_fmaf(o, second ? gB[t] : gA[t], rv[t]);
+          v[t] = o;
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(mxm_st4, pack8(v)), odesc, (int)ro[i], 0, 2);
+        ro[i] += ldo2;
+        asm volatile("" : "+v"(ro[i]));
+        if (EPI == WAN_EPI_GELU_TANH) __builtin_amdgcn_sched_barrier(0);  // 8 GELUs' temporaries at a time
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (tile >= end) break;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // trailing DMA (the LDS is released at the end)
 }
 
 }  // namespace
@@ -273,7 +336,7 @@ int wan_gemm_mxfp4m_try(const MxGemm& p, int epilogue, hipStream_t st) {
   if (256 * (int64_t)(p.K / 2) + 256 >= ((int64_t)1 << 31) || 256 * p.ldc * 2 + 512 >= ((int64_t)1 << 31)) return -1;   // 32-bit offsets inside a tile
   const int64_t ty = (p.M + MXM_BM - 1) / MXM_BM, tx = (p.N + MXM_BN - 1) / MXM_BN;
   if (ty * tx >= ((int64_t)1 << 31)) return -1;
-  const dim3 grid((unsigned)(ty * tx)), wg(256);
+  const dim3 grid((unsigned)min(ty * tx, (int64_t)256)), wg(256);   // one workgroup a CU
   const int group = epilogue == WAN_EPI_TRANSPOSED ? 8 : 4;
   switch (epilogue) {
     case WAN_EPI_NONE: hipLaunchKernelGGL(gemm_mxfp4m_kernel<WAN_EPI_NONE>, grid, wg, 0, st, p, (int)ty, (int)tx, group); break;

@@ -62,8 +62,8 @@ __device__ __forceinline__ mx_u4 mx_rsrc(const char* base, uint32_t bytes) {
 
 __device__ __forceinline__ float mx_gelu_tanh(float x) {
   const float c = -2.0f * 0.7978845608028654f * 1.4426950408889634f;  // -2 sqrt(2/pi) log2(e)
-  const float t = __builtin_fmaf(x * x, 0.044715f, 1.0f);
-  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * t * c));
+  const float t = __builtin_fmaf(x * x, 0.044715f * c, c);
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * t));
 }
 
 }  // namespace
