@@ -172,7 +172,9 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   MxmFrags f0, f1;
 #pragma unroll
   for (int r = 0; r < 16; ++r) load_frag(f0, ybw[0], xbw[0] + MXM_UNIT, ord(r));
-  uint32_t slot_y = 0;   // of the current stage
+  uint32_t slot_y = 0, slot_x = MXM_UNIT;   // of the current stage
+  uint32_t y1 = ybw[1], x1 = xbw[1] + MXM_UNIT, yn = 0, xn = 0;   // its k-step 1's fragments, the next stage's k-step 0's
+  mx_u4 ny = sy, nx = sx;   // the next stage's scales
   auto load_bias = [&](int64_t x) -> uint4 {   // of this lane's columns
     const int64_t c = x + wx * 128 + 8 * l15;
     return EPI != WAN_EPI_TRANSPOSED && p.bias != nullptr && c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.bias + c) : make_uint4(0u, 0u, 0u, 0u);
@@ -195,19 +197,23 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
     //   P_S: everything landed, stage S fully read + barrier
     //   MFMAs 16 .. 63: X_{S+2} -> slot of Y_S behind 16, 19, .., 37, Y_{S+3} -> slot of X_S behind 40, 43, .., 61; stage S + 1's first fragments
     //                   in the other gaps up to MFMA 39
+    // What a stage leaves to the next one is moved in the gaps too: between the stages it would hold the MFMAs up.
 #pragma unroll 1
     for (int k = 0; k < nk; ++k) {
-      const uint32_t slot_x = next_slot(slot_y), next_y = next_slot(slot_x), next_x = next_slot(next_y);
-      const uint32_t y1 = ybw[1] + slot_y, x1 = xbw[1] + slot_x, yn = ybw[0] + next_y, xn = xbw[0] + next_x;
-      mx_u4 ny, nx;
+      uint32_t next_y, next_x;
       mxm_run<0, 0, 64>(acc, f0, sy, sx, [&](int m) __attribute__((always_inline)) {
         if (m == 0) {
+          sy[2] = ny[2]; sy[3] = ny[3]; sx[2] = nx[2]; sx[3] = nx[3];
           ny = scale_of(ss.y);
           nx = scale_of(ss.x);
         }
         if ((m & 1) == 1 && m < 32) load_frag(f1, y1, x1, ord(m >> 1));
+        if (m == 34) next_y = next_slot(slot_x);
+        if (m == 36) next_x = next_slot(next_y);
+        if (m == 38) { yn = ybw[0] + next_y; xn = xbw[0] + next_x; }
+        if (m == 40) { y1 = ybw[1] + next_y; x1 = xbw[1] + next_x; }
+        if (m == 44) advance_scales(ss);
       });
-      advance_scales(ss);
       mxm_run<1, 0, 16>(acc, f1, sy, sx, [](int) {});
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -217,13 +223,14 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
         if (r == 0 && q < 8) piece(xs, slot_y, q);
         if (r == 0 && q >= 8) piece(ys, slot_x, q - 8);
         if (r != 0 && q < 8) load_frag(f0, yn, xn, ord(2 * q + r - 1));
+        if (m == 42) advance(xs, false);
+        if (m == 45) { sy[0] = ny[0]; sy[1] = ny[1]; sx[0] = nx[0]; sx[1] = nx[1]; }
+        if (m == 62) {
+          advance(ys, true);
+          slot_y = next_y;
+          slot_x = next_x;
+        }
       });
-      advance(xs, false);
-      advance(ys, true);
-      slot_y = __builtin_amdgcn_readfirstlane(next_y);
-      sy = ny;
-      sx = nx;
-      asm volatile("s_nop 1" : "+v"(sy), "+v"(sx)); /* a register copy in front of an MFMA that reads it: hipcc pads nothing around asm */
     }
     // the last MFMAs -> accumulator reads
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
