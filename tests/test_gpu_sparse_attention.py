@@ -296,6 +296,106 @@ def test_long_cache_past_32_bit_offsets(ops):
         assert ((m[0, :, j].to(F64) - ref).abs() <= 2.0 ** -24 * ref.abs() * 1.0001).all()
 
 
+# ---- up to 16 queries: a kernel of their own ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,Bk,H,Hk,Lq,Lk,keep,lens", [(1, 1, 1, 1, 1, 1, 1, None), (2, 1, 6, 2, 2, 65, 3, None), (2, 2, 5, 1, 15, 2000, 31, [2000, 63]), (1, 1, 40, 8, 16, 9000, 141, [8999]),
+                                                       (1, 1, 40, 8, 17, 9000, 141, [8999]), (3, 3, 400, 4, 1, 640, 9, [1, 64, 640]), (1, 1, 1, 1, 1, 75600, 1182, None),
+                                                       (1, 1, 4, 2, 7, 16000, 250, None), (1, 1, 1, 1, 5, 256, 4, None), (1, 1, 1, 1, 5, 320, 5, None)])
+def test_few_queries(ops, B, Bk, H, Hk, Lq, Lk, keep, lens):
+    """Both sides of the limit; one workgroup to a list and many, one block a wave and several; in place, strided, with counts."""
+    g = gen(Lq * 7 + keep)
+    fused = rnd(g, B, Lq, H, 2, 128)
+    q, k, v = fused[:, :, :, 0].contiguous(), rnd(g, Bk, Lk, Hk + 1, 128)[:, :, :Hk], rnd(g, Bk, Lk, Hk, 128)
+    index = lists(g, B, H, 1, (Lk + 63) // 64, keep)
+    count = torch.randint(0, keep + 2, (B, H, 1), generator=g, device="cuda", dtype=torch.int32)
+    vt = vt_of(v, fill=float("nan"))
+    clean = vt_of(v)
+    check(ops.sparse_attention(q, k, vt, index, k_lens=lens_of(lens)), *attend_ref(q, k, clean, index, None, lens))
+    got = ops.sparse_attention(q, k, vt, index, count, k_lens=lens_of(lens))
+    check(got, *attend_ref(q, k, clean, index, count, lens))
+    assert (got.permute(0, 2, 1, 3)[count[:, :, 0] == 0] == 0).all()
+    assert ops.sparse_attention(q, k, vt, index, count, k_lens=lens_of(lens), out=q) is q and torch.equal(q, got)
+
+
+@pytest.mark.parametrize("Lq", [1, 16])
+def test_few_queries_masked_places_may_hold_anything(ops, Lq):
+    g = gen(21)
+    lens = [70, 700, 0]
+    q, k, v = rnd(g, 3, Lq, 2, 128), rnd(g, 3, 1000, 2, 128), rnd(g, 3, 1000, 2, 128)
+    for b in range(3):
+        k[b, lens[b]:] = float("nan")
+        v[b, lens[b]:] = float("inf")
+        k[b, lens[b] + 1 :: 2] = -float("inf")
+    vt = vt_of(v, fill=float("nan"))
+    index = torch.tensor([-1, 15, 1, 0, 99, 1 << 30, -(1 << 31), 10, 3], dtype=torch.int32, device="cuda").expand(3, 2, 1, 9).contiguous()
+    got = ops.sparse_attention(q, k, vt, index, k_lens=lens_of(lens))
+    check(got, *attend_ref(q, torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(vt, 0, 0, 0), index, None, lens))
+    assert (got[2] == 0).all()
+
+
+def test_few_queries_keep_a_nan_that_is_attended(ops):
+    g = gen(22)
+    q, k, v = rnd(g, 1, 3, 1, 128), rnd(g, 1, 640, 1, 128), rnd(g, 1, 640, 1, 128)
+    k[0, 70, 0, 5] = float("nan")
+    vt = vt_of(v)
+    for entries in ([1], [1, 0], [0, 1, 2, 3, 4, 5, 6, 7, 8, 9]):
+        index = torch.tensor(entries, dtype=torch.int32, device="cuda").view(1, 1, 1, -1)
+        assert torch.isnan(ops.sparse_attention(q, k, vt, index)).all()
+    index = torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda").view(1, 1, 1, -1)
+    check(ops.sparse_attention(q, k, vt, index), *attend_ref(q, torch.nan_to_num(k), vt, index))
+
+
+def test_few_queries_maxima_that_rise_along_the_list(ops):
+    g = gen(23)
+    for sign in (1, -1):
+        k = rnd(g, 1, 19200, 1, 128, gain=0.02)
+        k[0, :, 0, 0] += (torch.arange(19200, device="cuda") // 64 * 2 * sign).to(BF)
+        q = rnd(g, 1, 9, 1, 128, gain=0.1)
+        q[0, :, 0, 0] = 8.0
+        q[0, ::3, 0, 0] = -8.0
+        v = rnd(g, 1, 19200, 1, 128)
+        index = torch.arange(300, dtype=torch.int32, device="cuda").view(1, 1, 1, 300)
+        vt = vt_of(v)
+        qs = (q.float() * ops.attention_qscale()).to(BF)
+        check(ops.sparse_attention(qs, k, vt, index, q_prescaled=True), *attend_ref(qs, k, vt, index, scale=math.log(2.0)))
+
+
+def test_few_queries_captured_beside_another_graph(ops):
+    g = gen(24)
+    state = []
+    for n in range(2):
+        q, k, v = rnd(g, 1, 1, 8, 128), rnd(g, 1, 4000, 2, 128), rnd(g, 1, 4000, 2, 128)
+        vt, index = vt_of(v), lists(g, 1, 8, 1, 63, 40)
+        ops.sparse_attention(q, k, vt, index)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.sparse_attention(q, k, vt, index)
+        state.append((graph, q, k, vt, index, out))
+    for turn in range(3):
+        for graph, q, *_ in state:
+            q.copy_(rnd(g, 1, 1, 8, 128))
+        for graph, *_ in state:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, q, k, vt, index, out in state:
+            assert torch.equal(out, ops.sparse_attention(q, k, vt, index))
+
+
+def test_long_cache_past_32_bit_offsets_of_many_queries(ops):
+    g = gen(25)
+    Lk, H = 430000, 40
+    k = torch.zeros(1, Lk, H, 128, dtype=BF, device="cuda")
+    vt = torch.zeros(1, H * 128, (Lk + 63) // 64 * 64, dtype=BF, device="cuda")
+    q = rnd(g, 1, 130, H, 128)
+    nk = (Lk + 63) // 64
+    index = torch.tensor([0, nk - 2, nk - 1], dtype=torch.int32, device="cuda").expand(1, H, 2, 3).contiguous()
+    for j in (0, nk - 2, nk - 1):
+        n = min(64, Lk - 64 * j)
+        k[0, 64 * j : 64 * j + n] = rnd(g, n, H, 128)
+        vt[0, :, 64 * j : 64 * j + n] = rnd(g, H * 128, n)
+    check(ops.sparse_attention(q, k, vt, index), *attend_ref(q, k, vt, index))
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------------------
 def test_pay_sparse_attention(ops):
     g = gen(16)

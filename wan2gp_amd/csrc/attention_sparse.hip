@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int Q_BLOCK = 128;
+constexpr int Q_BLOCK = 128, FEW = 16;
 constexpr float LAZY = 32.f;   // how far above its reference (log2) a row's scores may lie
 constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 
@@ -309,7 +309,8 @@ struct SparseArgs {
   int B, Bk, H, Hk, nq, keep;
   int q_prescaled;
   int parts;
-  float* part;    // parts > 1: [list][part][128 rows][128] sums, behind them [list][part][128 rows] {reference, row sum}
+  int rows;       // of a list in part
+  float* part;    // parts > 1: [list][part][rows][128] sums, behind them [list][part][rows] {reference, row sum}
 };
 
 // PARTS: a list is cut into `parts` workgroups' shares, which leave unnormalised sums for sparse_join_kernel
@@ -494,22 +495,172 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     }
 }
 
+// ---- up to 16 queries ------------------------------------------------------------------------------------------------------------------------
+// A token, or a handful: the cache's bytes and the latency are all there is.  A wave takes a block of 64 keys by itself, K and V^T straight from memory in
+// the operands' layouts (the permuted key order of above: 16 rows x 64 bytes a load of K, 16 x 64 of V^T), all 32 KB of it in flight at once, and a
+// workgroup's four waves join their sums in the LDS.  A list is cut into as many workgroups as leave a wave one block, up to 1,024 in all, then
+// sparse_join_kernel as above.
+// Bound by latency and by the way the bytes lie (rows of 256 bytes, of V^T 128): a token of 40 heads (8 of the cache) against 32 blocks each, 42 MB, in 12.7 us and 4
+// for the join, the kernel above 18 and 5.  16 queries there: 17.7 and 23.5 us; 12 heads, 148 blocks each: 25.9 and 31.6; 1 head, 1,182: 38.8 and 67.0; 40 heads of their own
+// caches, 148: 49.0 and 45.2; one query of 40 heads, 590: 112 and 114.
+__global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
+  __shared__ __attribute__((aligned(16))) float sum[4][FEW][132];
+  __shared__ float2 stat[4][FEW];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wg = blockIdx.x, id = wg / p.parts, pt = wg - id * p.parts;
+  const int b = id / p.H, h = id - b * p.H, bk = b % p.Bk, hk = h / (p.H / p.Hk);
+  // (the first entry is read with the count and the length, not behind them)
+  const int* list = p.index + (int64_t)id * p.keep;
+  int e = pt * 4 + wave, next = list[min(e, p.keep - 1)];
+  int entries = p.keep;
+  if (p.count != nullptr) entries = min(entries, max(p.count[id], 0));
+  int len = (int)p.Lk;
+  if (p.k_lens != nullptr) len = min(len, max(p.k_lens[bk], 0));
+  const int nvalid = (len + KVBLK - 1) / KVBLK;
+
+  mfma_bf16x8 qf[4];
+  const bf16_t* qp = p.q + (int64_t)b * p.q_batch + (int64_t)min(n, (int)p.Lq - 1) * p.q_row + (int64_t)h * 128 + 8 * g;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
+    if (!p.q_prescaled) {   // (as above: rounded with the scale)
+      float f[8];
+      unpack8(w, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
+      w = pack8(f);
+    }
+    qf[ks] = __builtin_bit_cast(mfma_bf16x8, w);
+  }
+  const bf16_t* kb = p.k + (int64_t)bk * p.k_batch + (int64_t)hk * 128 + 8 * g;
+  const bf16_t* vb = p.vt + (((int64_t)bk * p.Hk + hk) * 128 + n) * p.ldv + 8 * g;
+  f32x4 acc[8];
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, ref = 0.f, l = 0.f;   // the row's maximum so far, what its weights are relative to (0 until there is a maximum), this lane's share of its sum
+  for (; e < entries; e += 4 * p.parts) {
+    const int blk = __builtin_amdgcn_readfirstlane(next);
+    next = list[min(e + 4 * p.parts, p.keep - 1)];
+    if ((uint32_t)blk >= (uint32_t)nvalid) continue;
+    const int rem = len - blk * KVBLK;   // keys from here on
+    mfma_bf16x8 kf[4][4], vf[8][2];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      const int key = min(32 * (kt >> 1) + 8 * (n >> 2) + 4 * (kt & 1) + (n & 3), rem - 1);   // (past the end: the last key again, masked below)
+      const bf16_t* kr = kb + ((int64_t)blk * KVBLK + key) * p.k_row;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) kf[kt][ks] = *reinterpret_cast<const mfma_bf16x8*>(kr + 32 * ks);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) vf[dt][c] = *reinterpret_cast<const mfma_bf16x8*>(vb + (int64_t)(16 * dt) * p.ldv + blk * (int64_t)KVBLK + 32 * c);
+    f32x4 s[4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], qf[ks], s[kt], 0, 0, 0);
+    }
+    if (rem < KVBLK) {   // scores of keys past the end, and their V, which may hold anything: 0 * anything has to be 0
+      const int lim = rem - 8 * g;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (32 * (kt >> 1) + 4 * (kt & 1) + i >= lim) s[kt][i] = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          u32x4 w = __builtin_bit_cast(u32x4, vf[dt][c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int left = lim - 32 * c - 2 * j;
+            const uint32_t x = w[j];
+            w[j] = left >= 2 ? x : left == 1 ? x & 0xffffu : 0u;
+          }
+          vf[dt][c] = __builtin_bit_cast(mfma_bf16x8, w);
+        }
+    }
+    float t = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t = fmaxf(t, s[kt][i]);
+    t = fmaxf(t, __shfl_xor(t, 16, 64));
+    t = fmaxf(t, __shfl_xor(t, 32, 64));
+    const float up = fmaxf(top, t);
+    ref = up == -INFINITY ? 0.f : up;
+    const float a = __builtin_amdgcn_exp2f(top - ref);
+    top = up;
+    l *= a;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) acc[dt] *= a;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(s[2 * c + (j >> 2)][j & 3] - ref);
+        l += w[j];
+      }
+      const mfma_bf16x8 pk = __builtin_bit_cast(mfma_bf16x8, pack8(w));
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt][c], pk, acc[dt], 0, 0, 0);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(&sum[wave][n][16 * dt + 4 * g]) = acc[dt];
+  if (g == 0) stat[wave][n] = make_float2(l == 0.f ? -INFINITY : ref, l);
+  __syncthreads();
+  const int row = tid >> 4, col = (tid & 15) * 8;
+  if (row >= p.Lq) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, stat[w][row].x);
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 ml = stat[w][row];
+    const float a = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - m);
+    l += ml.y * a;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] += sum[w][row][col + j] * a;
+  }
+  if (p.parts > 1) {
+    float* d = p.part + ((int64_t)wg * p.rows + row) * 128 + col;
+    *reinterpret_cast<float4*>(d) = make_float4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<float4*>(d + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    if (col == 0) reinterpret_cast<float2*>(p.part + (int64_t)gridDim.x * p.rows * 128)[(int64_t)wg * p.rows + row] = make_float2(m, l);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;   // a row without keys: zeros
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] *= inv;
+  *reinterpret_cast<uint4*>(p.o + ((int64_t)b * p.Lq + row) * p.H * 128 + (int64_t)h * 128 + col) = pack8(o);
+}
+
 // o = sum of the parts' sums, each scaled from its own reference to the largest, over the row sums likewise: one wave per row, two columns a lane
 __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs) {
   const int id = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
   const int64_t r = (int64_t)qb * Q_BLOCK + row;
   if (r >= p.Lq) return;
-  const float2* st = reinterpret_cast<const float2*>(p.part + (int64_t)wgs * Q_BLOCK * 128) + (int64_t)id * p.parts * Q_BLOCK + row;
-  const float2 ml = lane < p.parts ? st[lane * Q_BLOCK] : make_float2(-INFINITY, 0.f);   // (at most 32 parts)
+  const float2* st = reinterpret_cast<const float2*>(p.part + (int64_t)wgs * p.rows * 128) + (int64_t)id * p.parts * p.rows + row;
+  const float2 ml = lane < p.parts ? st[lane * p.rows] : make_float2(-INFINITY, 0.f);   // (at most 64 parts)
   const float top = wave_max(ml.x);
   const float a = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
   const float l = wave_sum(ml.y * a);
-  const float* o = p.part + ((int64_t)id * p.parts * Q_BLOCK + row) * 128 + 2 * lane;
+  const float* o = p.part + ((int64_t)id * p.parts * p.rows + row) * 128 + 2 * lane;
   float s0 = 0.f, s1 = 0.f;
 #pragma unroll 8
   for (int k = 0; k < p.parts; ++k) {
-    const float2 v = *reinterpret_cast<const float2*>(o + (int64_t)k * Q_BLOCK * 128);
+    const float2 v = *reinterpret_cast<const float2*>(o + (int64_t)k * p.rows * 128);
     const float ak = __shfl(a, k, 64);
     s0 += v.x * ak;
     s1 += v.y * ak;
@@ -518,8 +669,15 @@ __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs)
   *reinterpret_cast<uint32_t*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 2 * lane) = cvt_pk(s0 * inv, s1 * inv);
 }
 
-// how many workgroups share a list: enough for two on every CU, a share no shorter than two blocks
-int sparse_parts(int64_t lists, int keep) {
+// How many workgroups share a list.  Few queries: one for every four blocks, up to 1,024 workgroups.  Else enough for two on every CU, a share no shorter than
+// two blocks.
+int sparse_parts(int64_t Lq, int64_t lists, int keep) {
+  if (Lq <= FEW) {
+    int64_t n = 1024 / lists;
+    if (n > (keep + 3) / 4) n = (keep + 3) / 4;
+    if (n > 64) n = 64;
+    return n < 2 ? 1 : (int)n;
+  }
   int64_t n = 512 / lists;
   if (n > keep / 2) n = keep / 2;
   if (n > 32) n = 32;
@@ -531,8 +689,8 @@ int sparse_parts(int64_t lists, int keep) {
 extern "C" int64_t wan_sparse_attention_scratch_bytes(int B, int64_t Lq, int H, int keep) {
   if (B < 1 || Lq < 1 || H < 1 || keep < 1) return 0;
   const int64_t lists = (Lq + Q_BLOCK - 1) / Q_BLOCK * H * B;
-  const int parts = sparse_parts(lists, keep);
-  return parts == 1 ? 0 : lists * parts * Q_BLOCK * (128 + 2) * 4;
+  const int parts = sparse_parts(Lq, lists, keep);
+  return parts == 1 ? 0 : lists * parts * (Lq <= FEW ? FEW : Q_BLOCK) * (128 + 2) * 4;
 }
 
 extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_batch, const wan_bf16* k, int64_t k_row, int64_t k_batch, const wan_bf16* vt, wan_bf16* o,
@@ -551,15 +709,20 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   const int64_t nq = (Lq + Q_BLOCK - 1) / Q_BLOCK;
   WAN_REQUIRE(nq * H * B < ((int64_t)1 << 31), "wan_sparse_attention: grid too large");
   const int64_t lists = nq * H * B;
-  const int parts = sparse_parts(lists, keep);
+  const int parts = sparse_parts(Lq, lists, keep);
   const int64_t need = wan_sparse_attention_scratch_bytes(B, Lq, H, keep);
   WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_sparse_attention: needs 16-byte aligned scratch of %lld bytes", (long long)need);
   hipStream_t st = as_stream(stream);
-  const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, parts, reinterpret_cast<float*>(scratch)};
-  if (parts == 1) {
+  const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, parts, Lq <= FEW ? FEW : Q_BLOCK, reinterpret_cast<float*>(scratch)};
+  if (Lq <= FEW) {
+    hipLaunchKernelGGL(attn_sparse_few_kernel, dim3((unsigned)(lists * parts)), dim3(256), 0, st, a);
+  } else if (parts == 1) {
     hipLaunchKernelGGL(attn_sparse_kernel<false>, dim3((unsigned)lists), dim3(128), 0, st, a);
   } else {
     hipLaunchKernelGGL(attn_sparse_kernel<true>, dim3((unsigned)(lists * parts)), dim3(128), 0, st, a);
+  }
+  if (parts > 1) {
+    WAN_LAUNCH_CHECK();
     const int64_t rows = Lq < Q_BLOCK ? Lq : Q_BLOCK;
     hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)lists, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (int)(lists * parts));
   }
