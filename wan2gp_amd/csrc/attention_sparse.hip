@@ -24,8 +24,12 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //   * the tiles' addresses come from the list, one scalar load a tile ahead of its use;
 //   * the softmax needs no bound on the scores: a half's maximum is taken (v_max3) between its last S tile and its first exp2, and only a score 2^LAZY
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
+//   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
+//     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.9 ms, 1.13 PFLOP/s, the matrix pipe busy for 58 % of the cycles at 1.9 GHz, the waves
+// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 733 us.
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
-// MFMA 0); a score is summed in the odd gap behind the next one's exp2, a pair packed in the odd gap behind its second; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
+// MFMA 0); a score is multiplied in the odd gap in front of its exp2 and summed in the one behind the next one's, a pair packed in the odd gap behind its second; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
 // t + 2 in every eighth gap, K from 3, V^T from 65 (the m0 of each in the gap in front of it): 64 pieces of 1 KB a CU and tile keep the path into the LDS
 // busy for 1,024 cycles, and issued in a row they hold up the waves; V^T(t) fragments 41 .. 71, K(t + 1) fragments 67 .. 97; the
 // addresses of tile t + 3 in the even gaps 112 .. 124.
@@ -34,6 +38,7 @@ struct SHalf {
   f32x4 accO[8][2];   // O^T tiles [d tile][q tile]
   f32x4 s[4][2];      // S^T - m [kv tile][q tile]
   u32x4 pk[4];        // P^T fragments, f = 2 c + q tile
+  float t;            // the score whose exp2 is next
   float p0, p1;       // the exp2 pair whose pack is pending
   float l[2], top[2]; // this lane's share of the row sums; maxima of the current tile
 };
@@ -61,9 +66,13 @@ __device__ __forceinline__ float sp_score(const SHalf& x, int k) {
   const int f = k >> 3;
   return x.s[2 * (f >> 1) + ((k >> 2) & 1)][f & 1][k & 3];
 }
+__device__ __forceinline__ void sp_scale(SHalf& x, int k, float scale) {
+  x.t = sp_score(x, k) * scale;
+  asm volatile("" : "+v"(x.t));
+}
 __device__ __forceinline__ void sp_exp(SHalf& x, int k) {
   float& p = (k & 1) ? x.p1 : x.p0;
-  p = __builtin_amdgcn_exp2f(sp_score(x, k));
+  p = __builtin_amdgcn_exp2f(x.t);
   asm volatile("" : "+v"(p));
 }
 __device__ __forceinline__ void sp_pack(SHalf& x, int k) {   // behind the odd score k
@@ -106,7 +115,7 @@ __device__ __forceinline__ void sp_maxes(SHalf& x) {
 // What leaves the straight path: the scores of a tile's keys past the end become -inf, and a row's reference moves to its maximum -- for the first
 // time (the row sum is 0: until a key has a finite score the reference is 0 and waits), or because a score lies more than 2^LAZY above it.
 // Returns whether a row still waits.
-__device__ __forceinline__ int sp_cold(SHalf& x, f32x4* negm, int rem) {
+__device__ __forceinline__ int sp_cold(SHalf& x, f32x4* negm, int rem, float scale, float lazy) {
   bool open = false;
   const int lim = rem - 8 * (int)(sp_lane() >> 4);
 #pragma unroll
@@ -127,8 +136,8 @@ __device__ __forceinline__ int sp_cold(SHalf& x, f32x4* negm, int rem) {
     l += __shfl_xor(l, 32, 64);
     const bool first = l == 0.f, none = t == -INFINITY;
     open |= first && none;
-    if (none || (!first && t <= LAZY)) t = 0.f;
-    const float a = __builtin_amdgcn_exp2f(-fmaxf(t, 0.f));   // (a first reference below 0: there is nothing to scale yet)
+    if (none || (!first && t <= lazy)) t = 0.f;
+    const float a = __builtin_amdgcn_exp2f(-fmaxf(t, 0.f) * scale);   // (a first reference below 0: there is nothing to scale yet)
     x.l[qt] *= a;
 #pragma unroll
     for (int i = 0; i < 4; ++i) negm[qt][i] -= t;
@@ -195,6 +204,7 @@ __device__ __forceinline__ void sp_load(SpList& d) {
 // lane offset and a scalar one; those of K, whose rows past the last key have to fail the range check, are lane offsets as a whole
 struct SpDma {
   uint32_t kofs[8], vofs, lds0, ldv2;
+  float scale, lazy;   // of the scores, in front of exp2; LAZY in their unit
 };
 // Two statements: the LDS address goes into m0 a gap ahead (nothing that hipcc emits in a tile touches m0; together they need an s_nop between them).  The
 // sum is made on the way into m0: forty of them kept in scalar registers did not fit.
@@ -283,19 +293,24 @@ __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], c
     if constexpr (G >= 29 && G <= 51) sp_maxes<(G - 29) / 2>(a);
     if constexpr (G >= 93 && G <= 115) sp_maxes<(G - 93) / 2>(b);
     if constexpr (G == 51) {
-      const uint64_t need = __ballot(fmaxf(a.top[0], a.top[1]) > LAZY) | (uint64_t)(force_a | (d.rem0 < KVBLK));
+      const uint64_t need = __ballot(fmaxf(a.top[0], a.top[1]) > m.lazy) | (uint64_t)(force_a | (d.rem0 < KVBLK));
       if (__builtin_expect(need != 0, 0)) {
         asm volatile("" ::: "memory");
-        force_a = sp_cold(a, &negm[0], d.rem0);
+        force_a = sp_cold(a, &negm[0], d.rem0, m.scale, m.lazy);
       }
     }
     if constexpr (G == 115) {
-      const uint64_t need = __ballot(fmaxf(b.top[0], b.top[1]) > LAZY) | (uint64_t)(force_b | (d.rem0 < KVBLK));
+      const uint64_t need = __ballot(fmaxf(b.top[0], b.top[1]) > m.lazy) | (uint64_t)(force_b | (d.rem0 < KVBLK));
       if (__builtin_expect(need != 0, 0)) {
         asm volatile("" ::: "memory");
-        force_b = sp_cold(b, &negm[2], d.rem0);
+        force_b = sp_cold(b, &negm[2], d.rem0, m.scale, m.lazy);
       }
     }
+    // the score whose exp2 is next
+    if constexpr (G <= 49) sp_scale(b, 6 + (G + 1) / 2, m.scale);
+    else if constexpr (G <= 113) sp_scale(a, (G - 51) / 2, m.scale);
+    else if constexpr (G <= 125) sp_scale(b, (G - 115) / 2, m.scale);
+    else sp_scale(b, 6, m.scale);
   }
   SB();
   if constexpr (G < 127) sp_slot<KS, VS, G + 1>(lds, kaddr, vaddr, qf, negm, kf, vf, a, b, m, d, force_a, force_b);
@@ -359,6 +374,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       for (int kt = 0; kt < 4; ++kt) x[c].s[kt][qt] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // (b's weights "of the tile before" the first: zeros)
     }
     x[c].p0 = x[c].p1 = 0.f;
+    x[c].t = -INFINITY;
 #pragma unroll
     for (int f = 0; f < 4; ++f) x[c].pk[f] = u32x4{0u, 0u, 0u, 0u};
   }
@@ -372,6 +388,8 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     SpDma m;
     m.lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 1024;
     m.ldv2 = uni((uint32_t)(p.ldv * 2));
+    m.scale = __uint_as_float(uni(__float_as_uint(p.q_prescaled ? 1.f : SPARSE_SCALE_LOG2E)));
+    m.lazy = __uint_as_float(uni(__float_as_uint(p.q_prescaled ? LAZY : LAZY / SPARSE_SCALE_LOG2E)));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t r = 8u * (i & 1) + ((uint32_t)tid >> 4), kt = i >> 1;   // LDS row 16 kt + r
@@ -394,15 +412,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
-        if (!p.q_prescaled) {   // the scale folded into q and rounded with it (as the dense kernels do): no multiplication per score
-          float f[8];
-          unpack8(w, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
-          w = pack8(f);
-        }
-        qf[qt][ks] = __builtin_bit_cast(mfma_bf16x8, w);
+        qf[qt][ks] = *reinterpret_cast<const mfma_bf16x8*>(qp + 32 * ks);
         asm volatile("" : "+a"(qf[qt][ks]));
       }
     }
@@ -450,6 +460,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     sp_sum(x[1], 5);
 #pragma unroll
     for (int k = 6; k < 32; ++k) {
+      if (k > 6) sp_scale(x[1], k, m.scale);
       sp_exp(x[1], k);
       asm volatile("s_nop 1");   // (no MFMA between the exp2 and its use here)
       sp_sum(x[1], k);
@@ -477,7 +488,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
         for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<float4*>(o + 16 * dt) = make_float4(x[c].accO[dt][qt][0], x[c].accO[dt][qt][1], x[c].accO[dt][qt][2], x[c].accO[dt][qt][3]);
         if (ge == 0) {
           float2* st = reinterpret_cast<float2*>(p.part + (int64_t)gridDim.x * Q_BLOCK * 128) + (int64_t)wg * Q_BLOCK + row;
-          *st = make_float2(l == 0.f ? -INFINITY : -negm[2 * c + qt][0], l);
+          *st = make_float2(l == 0.f ? -INFINITY : -negm[2 * c + qt][0] * (p.q_prescaled ? 1.f : SPARSE_SCALE_LOG2E), l);
         }
         continue;
       }
@@ -500,7 +511,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
 // the operands' layouts (the permuted key order of above: 16 rows x 64 bytes a load of K, 16 x 64 of V^T), all 32 KB of it in flight at once, and a
 // workgroup's four waves join their sums in the LDS.  A list is cut into as many workgroups as leave a wave one block, up to 1,024 in all, then
 // sparse_join_kernel as above.
-// Bound by latency and by the way the bytes lie (rows of 256 bytes, of V^T 128): a token of 40 heads (8 of the cache) against 32 blocks each, 42 MB, in 12.7 us and 4
+// Bound by latency and by the way the bytes lie (rows of 256 bytes, of V^T 128): a token of 40 heads (8 of the cache) against 32 blocks each, 42 MB, in 12.6 us and 4
 // for the join, the kernel above 18 and 5.  16 queries there: 17.7 and 23.5 us; 12 heads, 148 blocks each: 25.9 and 31.6; 1 head, 1,182: 38.8 and 67.0; 40 heads of their own
 // caches, 148: 49.0 and 45.2; one query of 40 heads, 590: 112 and 114.
 __global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
@@ -522,17 +533,8 @@ __global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
   mfma_bf16x8 qf[4];
   const bf16_t* qp = p.q + (int64_t)b * p.q_batch + (int64_t)min(n, (int)p.Lq - 1) * p.q_row + (int64_t)h * 128 + 8 * g;
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    uint4 w = *reinterpret_cast<const uint4*>(qp + 32 * ks);
-    if (!p.q_prescaled) {   // (as above: rounded with the scale)
-      float f[8];
-      unpack8(w, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= SPARSE_SCALE_LOG2E;
-      w = pack8(f);
-    }
-    qf[ks] = __builtin_bit_cast(mfma_bf16x8, w);
-  }
+  for (int ks = 0; ks < 4; ++ks) qf[ks] = *reinterpret_cast<const mfma_bf16x8*>(qp + 32 * ks);
+  const float scale = p.q_prescaled ? 1.f : SPARSE_SCALE_LOG2E;
   const bf16_t* kb = p.k + (int64_t)bk * p.k_batch + (int64_t)hk * 128 + 8 * g;
   const bf16_t* vb = p.vt + (((int64_t)bk * p.Hk + hk) * 128 + n) * p.ldv + 8 * g;
   f32x4 acc[8];
@@ -562,6 +564,7 @@ __global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
       s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], qf[ks], s[kt], 0, 0, 0);
+      s[kt] *= scale;
     }
     if (rem < KVBLK) {   // scores of keys past the end, and their V, which may hold anything: 0 * anything has to be 0
       const int lim = rem - 8 * g;
