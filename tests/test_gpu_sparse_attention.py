@@ -296,6 +296,21 @@ def test_long_cache_past_32_bit_offsets(ops):
         assert ((m[0, :, j].to(F64) - ref).abs() <= 2.0 ** -24 * ref.abs() * 1.0001).all()
 
 
+@pytest.mark.parametrize("B,Bk,H,Hk,Lq,Lk,keep,lens", [(1, 1, 40, 8, 1700, 3000, 9, [2999]), (2, 1, 20, 20, 1665, 640, 4, [577]), (1, 1, 30, 1, 2300, 5000, 70, None),
+                                                       (1, 1, 32, 2, 2048, 1000, 12, None)])
+def test_more_lists_than_run_at_a_time(ops, B, Bk, H, Hk, Lq, Lk, keep, lens):
+    """Whole rounds of lists, and what is left behind them cut into shares (none, a few, many); in place and with counts too."""
+    g = gen(Lq + keep)
+    q, k, v = rnd(g, B, Lq, H, 128), rnd(g, Bk, Lk, Hk, 128), rnd(g, Bk, Lk, Hk, 128)
+    nq = (Lq + 127) // 128
+    index = lists(g, B, H, nq, (Lk + 63) // 64, keep)
+    count = torch.randint(0, keep + 1, (B, H, nq), generator=g, device="cuda", dtype=torch.int32)
+    vt = vt_of(v, fill=float("nan"))
+    got = ops.sparse_attention(q, k, vt, index, count, k_lens=lens_of(lens))
+    check(got, *attend_ref(q, k, vt_of(v), index, count, lens))
+    assert ops.sparse_attention(q, k, vt, index, count, k_lens=lens_of(lens), out=q) is q and torch.equal(q, got)
+
+
 # ---- up to 16 queries: a kernel of their own ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Bk,H,Hk,Lq,Lk,keep,lens", [(1, 1, 1, 1, 1, 1, 1, None), (2, 1, 6, 2, 2, 65, 3, None), (2, 2, 5, 1, 15, 2000, 31, [2000, 63]), (1, 1, 40, 8, 16, 9000, 141, [8999]),
                                                        (1, 1, 40, 8, 17, 9000, 141, [8999]), (3, 3, 400, 4, 1, 640, 9, [1, 64, 640]), (1, 1, 1, 1, 1, 75600, 1182, None),

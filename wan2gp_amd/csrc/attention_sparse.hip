@@ -26,7 +26,7 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
 //   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
 //     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
-// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.9 ms, 1.13 PFLOP/s, the matrix pipe busy for 58 % of the cycles at 1.9 GHz, the waves
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.7 ms, 1.16 PFLOP/s, the matrix pipe busy for 58 % of the cycles at 1.9 GHz, the waves
 // waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 733 us.
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
 // MFMA 0); a score is multiplied in the odd gap in front of its exp2 and summed in the one behind the next one's, a pair packed in the odd gap behind its second; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
@@ -324,19 +324,22 @@ struct SparseArgs {
   int B, Bk, H, Hk, nq, keep;
   int q_prescaled;
   int parts;
+  int whole;      // the first lists of a launch in parts that are not cut
   int rows;       // of a list in part
-  float* part;    // parts > 1: [list][part][rows][128] sums, behind them [list][part][rows] {reference, row sum}
+  float* part;    // parts > 1: [cut list][part][rows][128] sums, behind them [cut list][part][rows] {reference, row sum}
 };
 
-// PARTS: a list is cut into `parts` workgroups' shares, which leave unnormalised sums for sparse_join_kernel
+// PARTS: the lists from `whole` on are cut into `parts` workgroups' shares, which leave unnormalised sums for sparse_join_kernel
 template <bool PARTS>
 __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   __shared__ __attribute__((aligned(16))) char smem[5 * IMG];   // K 0, 1, V^T 0, 1, 2
   lds_cchar* lds = (lds_cchar*)smem;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wg = uni(xcd_remap(blockIdx.x, gridDim.x));   // an XCD gets runs of neighbouring blocks of queries of a head: their lists have much in common
-  const int id = PARTS ? uni(wg / p.parts) : wg, pt = PARTS ? wg - id * p.parts : 0;
+  // an XCD gets runs of neighbouring blocks of queries of a head: their lists have much in common
+  const bool cut = PARTS && (int)blockIdx.x >= p.whole;
+  const int wg = uni(PARTS ? (cut ? xcd_remap(blockIdx.x - p.whole, gridDim.x - p.whole) : xcd_remap(blockIdx.x, p.whole)) : xcd_remap(blockIdx.x, gridDim.x));
+  const int own = cut ? uni(wg / p.parts) : wg, id = cut ? uni(p.whole + own) : wg, pt = cut ? wg - own * p.parts : 0;
   const int bh = uni(id / p.nq), qb = id - bh * p.nq, b = uni(bh / p.H), h = bh - b * p.H;
   const int bk = uni(b % p.Bk), hk = uni(h / (p.H / p.Hk));
 
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   d.len = uni(len);
   d.nvalid = uni((len + KVBLK - 1) / KVBLK);
   int e0 = 0, e1 = entries;
-  if (PARTS) {
+  if (cut) {
     e0 = uni((int)((int64_t)entries * pt / p.parts));
     e1 = uni((int)((int64_t)entries * (pt + 1) / p.parts));
   }
@@ -481,13 +484,13 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       float l = x[c].l[qt];
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
-      if (PARTS) {
+      if (cut) {
         if ((int64_t)qb * Q_BLOCK + row >= p.Lq) continue;   // (one query of a block: its row alone, not 64 KB of sums)
         float* o = p.part + ((int64_t)wg * Q_BLOCK + row) * 128 + 4 * ge;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<float4*>(o + 16 * dt) = make_float4(x[c].accO[dt][qt][0], x[c].accO[dt][qt][1], x[c].accO[dt][qt][2], x[c].accO[dt][qt][3]);
         if (ge == 0) {
-          float2* st = reinterpret_cast<float2*>(p.part + (int64_t)gridDim.x * Q_BLOCK * 128) + (int64_t)wg * Q_BLOCK + row;
+          float2* st = reinterpret_cast<float2*>(p.part + (int64_t)(gridDim.x - p.whole) * Q_BLOCK * 128) + (int64_t)wg * Q_BLOCK + row;
           *st = make_float2(l == 0.f ? -INFINITY : -negm[2 * c + qt][0] * (p.q_prescaled ? 1.f : SPARSE_SCALE_LOG2E), l);
         }
         continue;
@@ -650,8 +653,8 @@ __global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
 
 // o = sum of the parts' sums, each scaled from its own reference to the largest, over the row sums likewise: one wave per row, two columns a lane
 __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs) {
-  const int id = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int bh = id / p.nq, qb = id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
+  const int id = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;   // id: of the lists that were cut
+  const int bh = (p.whole + id) / p.nq, qb = p.whole + id - bh * p.nq, b = bh / p.H, h = bh - b * p.H;
   const int64_t r = (int64_t)qb * Q_BLOCK + row;
   if (r >= p.Lq) return;
   const float2* st = reinterpret_cast<const float2*>(p.part + (int64_t)wgs * p.rows * 128) + (int64_t)id * p.parts * p.rows + row;
@@ -672,19 +675,23 @@ __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs)
   *reinterpret_cast<uint32_t*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 2 * lane) = cvt_pk(s0 * inv, s1 * inv);
 }
 
-// How many workgroups share a list.  Few queries: one for every four blocks, up to 1,024 workgroups.  Else enough for two on every CU, a share no shorter than
-// two blocks.
-int sparse_parts(int64_t Lq, int64_t lists, int keep) {
-  if (Lq <= FEW) {
-    int64_t n = 1024 / lists;
-    if (n > (keep + 3) / 4) n = (keep + 3) / 4;
-    if (n > 64) n = 64;
-    return n < 2 ? 1 : (int)n;
-  }
-  int64_t n = 512 / lists;
-  if (n > keep / 2) n = keep / 2;
-  if (n > 32) n = 32;
-  return n < 2 ? 1 : (int)n;
+// How a launch's lists are cut.  Up to 16 queries: one workgroup for every four blocks of a list, up to 1,024 in all.  Else 512 workgroups run at a time: what is
+// left of the lists behind whole rounds of 512 is cut into as many shares as fill a round, none shorter than two blocks.  (More shares than that cost more in partial
+// sums than they gain: 312 lists of 48 blocks 109 us whole, 137 in two shares each.)  516 lists of 64 blocks take 150 us so and 221 uncut, 612 lists 173 and 223, 756 lists
+// 206 and 225; 156 lists of 48 blocks in three shares 56, in two 61.
+struct SparsePlan {
+  int64_t whole, cut;
+  int parts;
+};
+SparsePlan sparse_plan(int64_t Lq, int64_t lists, int keep) {
+  const bool few = Lq <= FEW;
+  const int64_t whole = few ? 0 : lists / 512 * 512, cut = lists - whole;
+  int64_t n = cut > 0 ? (few ? 1024 : 512) / cut : 0;
+  const int64_t shares = few ? (keep + 3) / 4 : keep / 2, most = few ? 64 : 32;
+  if (n > shares) n = shares;
+  if (n > most) n = most;
+  if (n < 2) return {lists, 0, 1};
+  return {whole, cut, (int)n};
 }
 
 }  // namespace
@@ -692,8 +699,8 @@ int sparse_parts(int64_t Lq, int64_t lists, int keep) {
 extern "C" int64_t wan_sparse_attention_scratch_bytes(int B, int64_t Lq, int H, int keep) {
   if (B < 1 || Lq < 1 || H < 1 || keep < 1) return 0;
   const int64_t lists = (Lq + Q_BLOCK - 1) / Q_BLOCK * H * B;
-  const int parts = sparse_parts(Lq, lists, keep);
-  return parts == 1 ? 0 : lists * parts * (Lq <= FEW ? FEW : Q_BLOCK) * (128 + 2) * 4;
+  const SparsePlan pl = sparse_plan(Lq, lists, keep);
+  return pl.cut * pl.parts * (Lq <= FEW ? FEW : Q_BLOCK) * (128 + 2) * 4;
 }
 
 extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_batch, const wan_bf16* k, int64_t k_row, int64_t k_batch, const wan_bf16* vt, wan_bf16* o,
@@ -710,24 +717,25 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   // a tile's 64 key rows and its 128 rows of V^T are addressed with 32-bit offsets from the tile's own 64-bit base
   WAN_REQUIRE(k_row < ((int64_t)1 << 24) && ldv < ((int64_t)1 << 23), "wan_sparse_attention: a row of k of %lld elements or %lld keys exceed the kernel's offsets", (long long)k_row, (long long)ldv);
   const int64_t nq = (Lq + Q_BLOCK - 1) / Q_BLOCK;
-  WAN_REQUIRE(nq * H * B < ((int64_t)1 << 31), "wan_sparse_attention: grid too large");
+  WAN_REQUIRE(nq * H * B < ((int64_t)1 << 31) - 1024, "wan_sparse_attention: grid too large");
   const int64_t lists = nq * H * B;
-  const int parts = sparse_parts(Lq, lists, keep);
+  const SparsePlan pl = sparse_plan(Lq, lists, keep);
   const int64_t need = wan_sparse_attention_scratch_bytes(B, Lq, H, keep);
   WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_sparse_attention: needs 16-byte aligned scratch of %lld bytes", (long long)need);
   hipStream_t st = as_stream(stream);
-  const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, parts, Lq <= FEW ? FEW : Q_BLOCK, reinterpret_cast<float*>(scratch)};
+  const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, pl.parts, (int)pl.whole, Lq <= FEW ? FEW : Q_BLOCK, reinterpret_cast<float*>(scratch)};
+  const unsigned wgs = (unsigned)(pl.whole + pl.cut * pl.parts);
   if (Lq <= FEW) {
-    hipLaunchKernelGGL(attn_sparse_few_kernel, dim3((unsigned)(lists * parts)), dim3(256), 0, st, a);
-  } else if (parts == 1) {
-    hipLaunchKernelGGL(attn_sparse_kernel<false>, dim3((unsigned)lists), dim3(128), 0, st, a);
+    hipLaunchKernelGGL(attn_sparse_few_kernel, dim3(wgs), dim3(256), 0, st, a);
+  } else if (pl.cut == 0) {
+    hipLaunchKernelGGL(attn_sparse_kernel<false>, dim3(wgs), dim3(128), 0, st, a);
   } else {
-    hipLaunchKernelGGL(attn_sparse_kernel<true>, dim3((unsigned)(lists * parts)), dim3(128), 0, st, a);
+    hipLaunchKernelGGL(attn_sparse_kernel<true>, dim3(wgs), dim3(128), 0, st, a);
   }
-  if (parts > 1) {
+  if (pl.cut > 0) {
     WAN_LAUNCH_CHECK();
     const int64_t rows = Lq < Q_BLOCK ? Lq : Q_BLOCK;
-    hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)lists, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (int)(lists * parts));
+    hipLaunchKernelGGL(sparse_join_kernel, dim3((unsigned)pl.cut, (unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (int)(pl.cut * pl.parts));
   }
   WAN_LAUNCH_CHECK();
   return 0;
