@@ -212,6 +212,44 @@ def test_linear_is_exact_where_fp32_is(ops):
         assert torch.equal(ops.linear_mxfp4(x, *ops.mxfp4_quantize(w)).to(F64), y.to(BF).to(F64)), (M, N, K)
 
 
+@pytest.mark.parametrize("M,N,K", [(40000, 1288, 32), (40001, 1288, 288), (33000, 2000, 512), (30720, 2304, 800), (25000, 2312, 1312), (70000, 520, 1600)])
+def test_several_tiles_a_workgroup(ops, M, N, K):
+    """Small integers again, so that every place of every tile of a workgroup's run is held to the exact result: stages left over at a tile's end, edges in both
+    directions, all four epilogues."""
+    g = gen(M)
+    x = torch.randint(-1, 2, (M, K), generator=g, device="cuda").to(BF) * 2
+    w = torch.randint(-1, 2, (N, K), generator=g, device="cuda").to(BF) * 2
+    x[:, ::32] = 4; w[:, ::32] = 4
+    b = torch.randint(-8, 9, (N,), generator=g, device="cuda").to(BF)
+    r = torch.randint(-8, 9, (M, N), generator=g, device="cuda").to(BF)
+    mod = torch.randint(0, 3, (6, N), generator=g, device="cuda").to(BF)
+    xm, wm = ops.mxfp4_quantize(x), ops.mxfp4_quantize(w)
+    y = (x.float() @ w.float().t()).to(torch.float32) + b.float()                   # (whole numbers below 2^24: exact in any order)
+    assert torch.equal(ops.linear_mxfp4(None, *wm, b, x_mx=xm), y.to(BF))
+    assert torch.equal(ops.linear_mxfp4(None, *wm, b, epilogue=2, residual=r, mod=mod, e=mod * 0 + 1, gate_idx=3, x_mx=xm), (r.float() + y * (mod[3].float() + 1)).to(BF))
+    assert torch.equal(ops.linear_mxfp4(None, *wm, b, epilogue=3, x_mx=xm)[:, :M], y.to(BF).t())
+    gelu = torch.nn.functional.gelu(y.double(), approximate="tanh")
+    bound = 2.0 ** -18 * y.double().abs()
+    close(ops.linear_mxfp4(None, *wm, b, epilogue=1, x_mx=xm), gelu, bound + 2.0 ** -8 * (gelu.abs() + bound))
+
+
+def test_linears_on_streams_beside_each_other(ops):
+    g = gen(8)
+    cases = []
+    for M, N, K in ((3, 2048, 5120), (600, 1536, 1536), (9000, 2304, 512)):
+        x, xm, wm, xd, wd = operands(ops, g, M, N, K)
+        cases.append((x, wm, ops.linear_mxfp4(x, *wm)))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append([ops.linear_mxfp4(x, *wm) for x, wm, _ in cases for _ in range(3)])
+    torch.cuda.synchronize()
+    for per in outs:
+        assert all(torch.equal(o, cases[i // 3][2]) for i, o in enumerate(per))
+
+
 def test_captured_linears_of_two_graphs(ops):
     g = gen(7)
     state = []
