@@ -72,16 +72,16 @@ __device__ __forceinline__ uint64_t order_key(double s) {
 
 // keys[row][j], on v_mfma_f64_16x16x4_f64: lane (n, g) supplies A[n][g] (query block n) and B[g][n] (key block n) of a step; register i holds D[4 i + g][n].  A
 // sum's order is free, so step 4 s + e takes column 16 s + 4 g + e: a load of four floats a lane is 64 consecutive bytes of each row (32 consecutive floats a
-// lane read every line of the L2 four times: 223 us).  One wave per 16 query blocks x KEY_TILES tiles of
-// 16 key blocks; the query block's 32 doubles stay in registers, and the four waves of a workgroup read the same keys.  Bound by the fp64 matrix rate (a step 64
+// lane read every line of the L2 four times: 223 us).  One wave per 16 query blocks x `tiles` tiles of
+// 16 key blocks (even: eight, down to two where that leaves fewer than 2,048 waves: 24 heads x 13 x 512 take 5.0 us
+// with two, 14.1 with eight); the query block's 32 doubles stay in registers, and the four waves of a workgroup read the same keys.  Bound by the fp64 matrix rate (a step 64
 // cycles) and the conversions in front of it: 40 heads x 591 x 1,182 in 173 us, 41 TFLOP/s and 223 MB of scores written.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-constexpr int KEY_TILES = 8;
 __global__ __launch_bounds__(256) void block_score_kernel(const float* __restrict__ qm, const float* __restrict__ km, uint64_t* __restrict__ keys, int H, int Hk,
-                                                         int Bk, int nq, int nk) {
+                                                         int Bk, int nq, int nk, int tiles) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int bh = blockIdx.z, b = bh / H, h = bh - b * H;
-  const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 16, k0 = blockIdx.x * (16 * KEY_TILES);
+  const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 16, k0 = blockIdx.x * (16 * tiles);
   if (q0 >= nq) return;
   const float* qp = qm + ((int64_t)bh * nq + min(q0 + n, nq - 1)) * 128 + 4 * g;
   const float* kp = km + ((int64_t)(b % Bk) * Hk + h / (H / Hk)) * nk * 128 + 4 * g;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void block_score_kernel(const float* __restric
     a[s] = v.x; a[s + 1] = v.y; a[s + 2] = v.z; a[s + 3] = v.w;
   }
   // two tiles at a time: two independent chains of products, and twice the loads in flight
-  for (int t = 0; t < KEY_TILES && k0 + 16 * t < nk; t += 2) {
+  for (int t = 0; t < tiles && k0 + 16 * t < nk; t += 2) {
     float4 v[2][8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -286,8 +286,10 @@ extern "C" int wan_select_blocks(const float* q_mean, const float* k_mean, const
   WAN_REQUIRE((((uintptr_t)q_mean | (uintptr_t)k_mean) & 15) == 0, "wan_select_blocks: the means must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
   uint64_t* keys = reinterpret_cast<uint64_t*>(scratch);
-  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 16 * KEY_TILES - 1) / (16 * KEY_TILES)), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean,
-                     keys, H, Hk, Bk, (int)nq, (int)nk);
+  int tiles = 8;
+  while (tiles > 2 && (nk + 16 * tiles - 1) / (16 * tiles) * ((nq + 15) / 16) * B * H < 2048) tiles /= 2;
+  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 16 * tiles - 1) / (16 * tiles)), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean,
+                     keys, H, Hk, Bk, (int)nq, (int)nk, tiles);
   WAN_LAUNCH_CHECK();
   const int64_t rows = (int64_t)B * H * nq;
   const dim3 grid((unsigned)((rows + 3) / 4)), wg(256);
