@@ -183,13 +183,17 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   uint4 bias = load_bias((int64_t)at.x * MXM_BN);
   for (;;) {
     f32x4 acc[8][8];
+    {
+      float bcol[8];   // the sums start at the bias of their column: an addition an element less in the epilogue
+      unpack8(bias, bcol);
 #pragma unroll
-    for (int a = 0; a < 8; ++a)
+      for (int b = 0; b < 8; ++b)
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-        asm volatile("" : "+a"(acc[a][b]));
-      }
+        for (int a = 0; a < 8; ++a) {
+          acc[a][b] = f32x4{bcol[b], bcol[b], bcol[b], bcol[b]};
+          asm volatile("" : "+a"(acc[a][b]));
+        }
+    }
     asm volatile("s_nop 1" ::: "memory");   // (in front of the first MFMA that reads them: hipcc pads nothing around asm)
     // Stage S: Y in slot 2 S % 5, X in (2 S + 1) % 5 (S counted over the tiles).
     //   k-step 0 (f0): stage S + 1's scales behind MFMA 0, k-step 1's fragments behind MFMA 1, 3, .., 31
@@ -235,8 +239,6 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
     // the last MFMAs -> accumulator reads
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     const int64_t y0 = (int64_t)at.y * MXM_BM, x0 = (int64_t)at.x * MXM_BN;
-    float bcol[8];
-    unpack8(bias, bcol);
     tile += step;
     if (tile < end) {
       at = decode(tile);
@@ -315,7 +317,8 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
         const bool second = row_lane + rit >= rb;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-          float o = acc[a][t][i] + (EPI == WAN_EPI_TRANSPOSED ? brow : bcol[t]);
+          float o = acc[a][t][i];
+          if (EPI == WAN_EPI_TRANSPOSED) o += brow;
           if (EPI == WAN_EPI_GELU_TANH) o = mx_gelu_tanh(o);
           if (EPI == WAN_EPI_GATE_RES) o = __builtin_fmaf(o, second ? gB[t] : gA[t], rv[t]);
           v[t] = o;
