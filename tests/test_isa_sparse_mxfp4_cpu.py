@@ -88,8 +88,13 @@ def test_mxfp4_gemm_of_many_tiles(asm):
         assert meta["ScratchSize"] == 0 and meta["LDSByteSize"] == 160 * 1024 and meta["NumAgprs"] == 256, (name, meta)
         assert not written_in_front(lines), written_in_front(lines)[:4]
         ops = collections.Counter(l.split()[0] for l in lines)
-        assert ops["v_mfma_scale_f32_16x16x128_f8f6f4"] == 128, ops   # one stage body
-        assert ops["s_barrier"] == 2
+        assert ops["v_mfma_scale_f32_16x16x128_f8f6f4"] == 256, ops   # a tile's first stage and the others
+        assert ops["s_barrier"] == 3
+        # a tile's first stage waits for nothing younger than the 32 stores of the epilogue in front of it, and hipcc puts no full wait behind them
+        assert ops["buffer_store_dwordx4"] == 32
+        first = next(i for i, l in enumerate(lines) if l.startswith("s_waitcnt vmcnt(32) lgkmcnt(0)"))
+        store = max(i for i, l in enumerate(lines[:first]) if l.startswith("buffer_store"))
+        assert not [l for l in lines[store:first] if "vmcnt(0)" in l], name
 
 
 def test_mxfp4_gemm_of_few_tiles(asm):

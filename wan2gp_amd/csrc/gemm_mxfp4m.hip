@@ -4,8 +4,8 @@
 // units, fragment reads and register-direct stores carry over, and a k-step of 128 is 64 MFMAs of 16 cycles (v_mfma_scale_f32_16x16x128_f8f6f4 on
 // two fp4 operands) where gemm256m's of 32 is 64 MFMAs of 16 cycles -- four times the FLOP on the same bytes and issue slots.  What differs:
 //   * one workgroup a CU takes one tile after the other, and the streams of units run on into the next tile: its first stages land and this tile's stores
-//     drain while the other of the two is worked on (a workgroup a tile: 32,760 x 8,960 x 1,536 297 us, so 255; with the GELU 356 and 310).  The tile
-//     loop has one stage body with its ring slots in scalar registers.
+//     drain while the other of the two is worked on (a workgroup a tile: 32,760 x 8,960 x 1,536 297 us, so 242; with the GELU 356 and 292).  The tile
+//     loop has one stage body, and one more for a tile's first stage, with the ring slots in scalar registers.
 //   * both operands' image rows are (slab, t, n) = row slab * 128 + 8 n + t: a lane's eight scales of an operand and k-step are then 8 consecutive
 //     bytes of mxfp4_ops.hip's scale tiles, and all of a stage's one 16-byte load (dword 2 ks + (t >> 2), byte t & 3: the instruction picks the
 //     byte).  y tile a, register i of lane (n, g) is row 8 (4 g + i) + a.
@@ -15,11 +15,13 @@
 //     80 MFMAs (1,280 cycles) by then.
 //   * K need not be a multiple of 256: what a row's last stage reads past the row is the next row's codes (the buffer's end reads as zeros), and the
 //     scale bytes there are 0 on both sides -- (6 * 2^-127)^2 is 0 in fp32.
-//   * stores are non-temporal: 256 tiles are 32 MB, more than the L2 keeps for whoever reads them (with ordinary stores 268 us for 255 above).
-// Bound by the card's power where K is long: 75,600 x 5,120 x 13,824 with the gated residual in 2.34 ms, 4.6 PFLOP/s, 67 % of the cycles on the matrix pipe
+//   * stores are non-temporal: 256 tiles are 32 MB, more than the L2 keeps for whoever reads them (with ordinary stores 5 % slower).
+// Bound by the card's power where K is long: 75,600 x 5,120 x 13,824 with the gated residual in 2.17 - 2.30 ms by the card, 4.7 - 4.9 PFLOP/s, 67 % of the cycles on the matrix pipe
 // at 1.4 GHz; the same MFMAs with no memory access between them would take 1.75 ms.  Where K is short, by the epilogue: at K = 1,536 the GELU's
-// 52 VALU cycles an element are as much as the products' (310 us, 2.9 PFLOP/s).
+// 48 VALU cycles an element are as much as the products' (292 us, 3.1 PFLOP/s).
 #include "mxfp4.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -157,7 +159,9 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   enter(xs, tile, false);
   enter_scales(ss, tile);
   mx_u4 sy = scale_of(ss.y), sx = scale_of(ss.x);
-  asm volatile("" : "+v"(sy), "+v"(sx));
+  advance_scales(ss);
+  mx_u4 ny = scale_of(ss.y), nx = scale_of(ss.x);   // the next stage's
+  asm volatile("" : "+v"(sy), "+v"(sx), "+v"(ny), "+v"(nx));
   advance_scales(ss);
 #pragma unroll
   for (int u = 0; u < 5; ++u) {
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
     if (u & 1) advance(xs, false);
     else advance(ys, true);
   }
-  asm volatile("s_waitcnt vmcnt(24)" ::: "memory");  // stage 0 landed
+  asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // stages 0 and 1 landed
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   MxmFrags f0, f1;
@@ -174,13 +178,13 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
   for (int r = 0; r < 16; ++r) load_frag(f0, ybw[0], xbw[0] + MXM_UNIT, ord(r));
   uint32_t slot_y = 0, slot_x = MXM_UNIT;   // of the current stage
   uint32_t y1 = ybw[1], x1 = xbw[1] + MXM_UNIT, yn = 0, xn = 0;   // its k-step 1's fragments, the next stage's k-step 0's
-  mx_u4 ny = sy, nx = sx;   // the next stage's scales
   auto load_bias = [&](int64_t x) -> uint4 {   // of this lane's columns
     const int64_t c = x + wx * 128 + 8 * l15;
     return EPI != WAN_EPI_TRANSPOSED && p.bias != nullptr && c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.bias + c) : make_uint4(0u, 0u, 0u, 0u);
   };
   Tile at = decode(tile);
   uint4 bias = load_bias((int64_t)at.x * MXM_BN);
+  asm volatile("" : "+v"(bias.x), "+v"(bias.y), "+v"(bias.z), "+v"(bias.w));   // (waited for here: in the loop hipcc then waits for what is older than the stores)
   for (;;) {
     f32x4 acc[8][8];
     {
@@ -202,11 +206,13 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
     //   MFMAs 16 .. 63: X_{S+2} -> slot of Y_S behind 16, 19, .., 37, Y_{S+3} -> slot of X_S behind 40, 43, .., 61; stage S + 1's first fragments
     //                   in the other gaps up to MFMA 39
     // What a stage leaves to the next one is moved in the gaps too: between the stages it would hold the MFMAs up.
-#pragma unroll 1
-    for (int k = 0; k < nk; ++k) {
+    // A tile's first stage has its successor's scales and units from in front of the epilogue, and waits for no store of it: what is waited for is older than the
+    // 32 stores (in front of the first tile there are none, and nothing is waited for that has not landed).
+    auto stage = [&](auto is_first) __attribute__((always_inline)) {
+      constexpr bool FIRST = decltype(is_first)::value;
       uint32_t next_y, next_x;
       mxm_run<0, 0, 64>(acc, f0, sy, sx, [&](int m) __attribute__((always_inline)) {
-        if (m == 0) {
+        if (!FIRST && m == 0) {
           sy[2] = ny[2]; sy[3] = ny[3]; sx[2] = nx[2]; sx[3] = nx[3];
           ny = scale_of(ss.y);
           nx = scale_of(ss.x);
@@ -216,10 +222,11 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
         if (m == 36) next_x = next_slot(next_y);
         if (m == 38) { yn = ybw[0] + next_y; xn = xbw[0] + next_x; }
         if (m == 40) { y1 = ybw[1] + next_y; x1 = xbw[1] + next_x; }
-        if (m == 44) advance_scales(ss);
+        if (!FIRST && m == 44) advance_scales(ss);
       });
       mxm_run<1, 0, 16>(acc, f1, sy, sx, [](int) {});
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      if (FIRST) asm volatile("s_waitcnt vmcnt(32) lgkmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" : "+v"(ny), "+v"(nx)::"memory");
       mxm_run<1, 16, 64>(acc, f1, sy, sx, [&](int m) __attribute__((always_inline)) {
@@ -235,9 +242,16 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
           slot_x = next_x;
         }
       });
-    }
+    };
+    stage(std::true_type{});
+#pragma unroll 1
+    for (int k = 1; k < nk; ++k) stage(std::false_type{});
     // the last MFMAs -> accumulator reads
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    sy[2] = ny[2]; sy[3] = ny[3]; sx[2] = nx[2]; sx[3] = nx[3];
+    ny = scale_of(ss.y);
+    nx = scale_of(ss.x);
+    advance_scales(ss);
     const int64_t y0 = (int64_t)at.y * MXM_BM, x0 = (int64_t)at.x * MXM_BN;
     tile += step;
     if (tile < end) {
@@ -285,6 +299,11 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
       }
     }
     typedef unsigned int mxm_st4 __attribute__((__vector_size__(16)));
+    uint32_t brow[32] = {};   // the bias along the rows: all of it in front of the stores, which a load behind them would wait for
+    if (EPI == WAN_EPI_TRANSPOSED && pe->bias != nullptr) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r) brow[r] = pe->bias[min(y0 + row_lane + r, pe->M - 1)];
+    }
     uint32_t ro[4];   // rows 8 i + a of the current a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -310,15 +329,13 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t rit = (uint32_t)(8 * i + a);
-        float brow = 0.f;
-        if (EPI == WAN_EPI_TRANSPOSED && pe->bias != nullptr) brow = bf2f(pe->bias[min(y0 + row_lane + rit, pe->M - 1)]);
         float v[8], rv[8];
         if (EPI == WAN_EPI_GATE_RES) unpack8(rq[a % 3][i], rv);
         const bool second = row_lane + rit >= rb;
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
           float o = acc[a][t][i];
-          if (EPI == WAN_EPI_TRANSPOSED) o += brow;
+          if (EPI == WAN_EPI_TRANSPOSED) o += __uint_as_float(brow[rit] << 16);
           if (EPI == WAN_EPI_GELU_TANH) o = mx_gelu_tanh(o);
           if (EPI == WAN_EPI_GATE_RES) o = __builtin_fmaf(o, second ? gB[t] : gA[t], rv[t]);
           v[t] = o;
