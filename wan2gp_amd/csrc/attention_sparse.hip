@@ -26,10 +26,11 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
 //   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
 //     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
-// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.7 ms, 1.16 PFLOP/s, the matrix pipe busy for 58 % of the cycles at 1.9 GHz, the waves
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.4 ms, 1.18 PFLOP/s, the matrix pipe busy for 60 % of the cycles at 1.9 GHz, the waves
 // waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 733 us.
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
-// MFMA 0); a score is multiplied in the odd gap in front of its exp2 and summed in the one behind the next one's, a pair packed in the odd gap behind its second; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
+// MFMA 0); a score is multiplied in the odd gap in front of its exp2, a pair packed in the odd gap behind its second, fragments summed by one MFMA more behind
+// the last product of each; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
 // t + 2 in every eighth gap, K from 3, V^T from 65 (the m0 of each in the gap in front of it): 64 pieces of 1 KB a CU and tile keep the path into the LDS
 // busy for 1,024 cycles, and issued in a row they hold up the waves; V^T(t) fragments 41 .. 71, K(t + 1) fragments 67 .. 97; the
 // addresses of tile t + 3 in the even gaps 112 .. 124.
@@ -40,7 +41,8 @@ struct SHalf {
   u32x4 pk[4];        // P^T fragments, f = 2 c + q tile
   float t;            // the score whose exp2 is next
   float p0, p1;       // the exp2 pair whose pack is pending
-  float l[2], top[2]; // this lane's share of the row sums; maxima of the current tile
+  f32x4 l[2];         // the row sums (all four registers the same), on the matrix pipe: a row of ones as one more row of V^T
+  float top[2];       // maxima of the current tile
 };
 __device__ __forceinline__ void sp_qk0(f32x4& d, const mfma_bf16x8& k, const mfma_bf16x8& q, const f32x4& c) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %3" : "=&v"(d) : "v"(k), "a"(q), "v"(c));
@@ -80,12 +82,10 @@ __device__ __forceinline__ void sp_pack(SHalf& x, int k) {   // behind the odd s
   x.pk[j >> 2][j & 3] = cvt_pk(x.p0, x.p1);
   asm volatile("" : "+v"(x.pk[j >> 2]));
 }
-// score k's weight into its row's sum: a plain add, in front of the pack of its gap -- a compiler's instruction there is the wait state that hipcc would otherwise fill
-// with an s_nop, not counting the asm MFMA.  (v_dot2_f32_bf16 over the packed pair is half as many instructions and cost 400 cycles a tile more.)
-__device__ __forceinline__ void sp_sum(SHalf& x, int k) {
-  const int qt = (k >> 3) & 1;
-  x.l[qt] += (k & 1) ? x.p1 : x.p0;
-  asm volatile("" : "+v"(x.l[qt]));
+// fragment f's weights into their rows' sums.  (An addition per score costs 256 issue cycles a tile, these eight MFMAs 64; v_dot2_f32_bf16 over the packed pairs is as few
+// instructions as half the additions and cost 400 cycles a tile more.)
+__device__ __forceinline__ void sp_sum_step(SHalf& x, const mfma_bf16x8& ones, int f) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(x.l[f & 1]) : "v"(ones), "v"(__builtin_bit_cast(mfma_bf16x8, x.pk[f])));
 }
 // step j = 0 .. 7 of the maximum over a q tile's 16 scores, in the order the S tiles are finished
 template <int J>
@@ -131,10 +131,7 @@ __device__ __forceinline__ int sp_cold(SHalf& x, f32x4* negm, int rem, float sca
       }
     t = fmaxf(t, __shfl_xor(t, 16, 64));
     t = fmaxf(t, __shfl_xor(t, 32, 64));
-    float l = x.l[qt];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    const bool first = l == 0.f, none = t == -INFINITY;
+    const bool first = x.l[qt][0] == 0.f, none = t == -INFINITY;
     open |= first && none;
     if (none || (!first && t <= lazy)) t = 0.f;
     const float a = __builtin_amdgcn_exp2f(-fmaxf(t, 0.f) * scale);   // (a first reference below 0: there is nothing to scale yet)
@@ -256,12 +253,14 @@ __device__ __forceinline__ void sp_clean(char* img, int rem, int wave) {
 // the MFMA of gap G and what sits behind it; KS, VS: the images of tile t (K read already, V^T read here)
 template <int KS, int VS, int G>
 __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], const int (&vaddr)[2], const mfma_bf16x8 (&qf)[4][4], f32x4 (&negm)[4], mfma_bf16x8 (&kf)[4][4],
-                                        mfma_bf16x8 (&vf)[8][2], SHalf& a, SHalf& b, const SpDma& m, SpList& d, int& force_a, int& force_b) {
+                                        mfma_bf16x8 (&vf)[8][2], const mfma_bf16x8& ones, SHalf& a, SHalf& b, const SpDma& m, SpList& d, int& force_a, int& force_b) {
   constexpr int KN = (KS ^ 1) * IMG, VB = (2 + VS) * IMG;
   if constexpr (G < 32) sp_s_step(a, kf, qf, negm, 0, G);
   else if constexpr (G < 64) sp_pv_step(b, vf, G - 32);
   else if constexpr (G < 96) sp_s_step(b, kf, qf, negm, 2, G - 64);
   else sp_pv_step(a, vf, G - 96);
+  if constexpr (G >= 32 && G < 64 && (G & 7) == 7) sp_sum_step(b, ones, (G - 32) >> 3);
+  if constexpr (G >= 96 && (G & 7) == 7) sp_sum_step(a, ones, (G - 96) >> 3);
   SB();
   if constexpr ((G & 1) == 0) {
     if constexpr (G <= 50) sp_exp(b, 6 + G / 2);
@@ -275,12 +274,15 @@ __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], c
     if constexpr (G == 118) sp_apply_rows(d);
     if constexpr (G == 124) sp_apply_v(d);
   } else {
-    // the sum of the score before; behind an odd score its pair's pack
+    // behind an odd score its pair's pack
     constexpr int K = G <= 51 ? 6 + G / 2 : G <= 115 ? (G - 53) / 2 : (G - 117) / 2;
     SHalf& x = G > 51 && G <= 115 ? a : b;
-    if constexpr (K > 0) sp_sum(x, K - 1);
-    else if constexpr (G == 53) sp_sum(b, 31);
-    else sp_sum(a, 31);
+    // the score whose exp2 is next: in front of the pack, a compiler's instruction there is the wait state that hipcc would otherwise fill with an s_nop (it does not count
+    // the asm MFMA); where a tile may leave the straight path, behind that
+    if constexpr (G <= 49) sp_scale(b, 6 + (G + 1) / 2, m.scale);
+    else if constexpr (G == 127) sp_scale(b, 6, m.scale);
+    else if constexpr (G > 51 && G <= 113) sp_scale(a, (G - 51) / 2, m.scale);
+    else if constexpr (G > 115) sp_scale(b, (G - 115) / 2, m.scale);
     if constexpr ((K & 1) == 1) sp_pack(x, K);
     if constexpr (G >= 41 && G <= 55) vf[(G - 41) / 2][0] = *(lds_frag*)(lds + (VB + (G - 41) / 2 * 2048) + vaddr[0]);
     if constexpr (G >= 57 && G <= 71) vf[(G - 57) / 2][1] = *(lds_frag*)(lds + (VB + (G - 57) / 2 * 2048) + vaddr[1]);
@@ -306,14 +308,11 @@ __device__ __forceinline__ void sp_slot(lds_cchar* lds, const int (&kaddr)[4], c
         force_b = sp_cold(b, &negm[2], d.rem0, m.scale, m.lazy);
       }
     }
-    // the score whose exp2 is next
-    if constexpr (G <= 49) sp_scale(b, 6 + (G + 1) / 2, m.scale);
-    else if constexpr (G <= 113) sp_scale(a, (G - 51) / 2, m.scale);
-    else if constexpr (G <= 125) sp_scale(b, (G - 115) / 2, m.scale);
-    else sp_scale(b, 6, m.scale);
+    if constexpr (G == 51) sp_scale(a, 0, m.scale);
+    if constexpr (G == 115) sp_scale(b, 0, m.scale);
   }
   SB();
-  if constexpr (G < 127) sp_slot<KS, VS, G + 1>(lds, kaddr, vaddr, qf, negm, kf, vf, a, b, m, d, force_a, force_b);
+  if constexpr (G < 127) sp_slot<KS, VS, G + 1>(lds, kaddr, vaddr, qf, negm, kf, vf, ones, a, b, m, d, force_a, force_b);
 }
 
 struct SparseArgs {
@@ -366,7 +365,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       negm[2 * c + qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      x[c].l[qt] = 0.f;
+      x[c].l[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
       x[c].top[qt] = 0.f;
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) {
@@ -437,6 +436,8 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) kf[r & 3][r >> 2] = *(lds_frag*)(lds + (r & 3) * 4096 + kaddr[r >> 2]);
 
+    mfma_bf16x8 ones = __builtin_bit_cast(mfma_bf16x8, make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+    asm volatile("" : "+v"(ones));
     int force_a = 1, force_b = 1;   // a row without a reference is left
 #define SP_TILE(J)                                                                                                               \
     if (t + (J) >= nt) break;                                                                                                    \
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     __builtin_amdgcn_s_barrier();                                                                                                \
     asm volatile("" ::: "memory");                                                                                               \
     if (__builtin_expect(d.rem0 < KVBLK, 0)) sp_clean(smem + (2 + (J) % 3) * IMG, d.rem0, wave);                                  \
-    sp_slot<(J) & 1, (J) % 3, 0>(lds, kaddr, vaddr, qf, negm, kf, vf, x[0], x[1], m, d, force_a, force_b);                        \
+    sp_slot<(J) & 1, (J) % 3, 0>(lds, kaddr, vaddr, qf, negm, kf, vf, ones, x[0], x[1], m, d, force_a, force_b);                        \
     d.rem0 = d.rem1;                                                                                                             \
     d.rem1 = d.rem2;                                                                                                             \
     d.rem2 = d.rem3;
@@ -460,19 +461,19 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
     }
 #undef SP_TILE
     // b's last weights and products
-    sp_sum(x[1], 5);
 #pragma unroll
     for (int k = 6; k < 32; ++k) {
       if (k > 6) sp_scale(x[1], k, m.scale);
       sp_exp(x[1], k);
       asm volatile("s_nop 1");   // (no MFMA between the exp2 and its use here)
-      sp_sum(x[1], k);
       if (k & 1) sp_pack(x[1], k);
     }
     asm volatile("s_nop 7" ::: "memory");
     SB();
 #pragma unroll
     for (int i = 0; i < 32; ++i) { sp_pv_step(x[1], vf, i); SB(); }
+#pragma unroll
+    for (int f = 0; f < 4; ++f) { sp_sum_step(x[1], ones, f); SB(); }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");   // trailing DMA (the LDS is released at the end); the last MFMAs -> accumulator reads
   }
   const int lane_e = (int)sp_lane(), ne = lane_e & 15, ge = lane_e >> 4;
@@ -481,9 +482,7 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       const int row = wave * 64 + 32 * c + 16 * qt + ne;
-      float l = x[c].l[qt];
-      l += __shfl_xor(l, 16, 64);
-      l += __shfl_xor(l, 32, 64);
+      const float l = x[c].l[qt][0];
       if (cut) {
         if ((int64_t)qb * Q_BLOCK + row >= p.Lq) continue;   // (one query of a block: its row alone, not 64 KB of sums)
         float* o = p.part + ((int64_t)wg * Q_BLOCK + row) * 128 + 4 * ge;
