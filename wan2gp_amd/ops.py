@@ -324,8 +324,9 @@ def attention_sp(q, k_local, vt_local, k_all, vt_all, own_seg, out=None):
 
 
 def _same_device(first, *others):
+    d = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
             raise _L.WanHipError(f"all tensors must be on one device, got {first.device} and {t.device}")
 
 
@@ -337,7 +338,7 @@ def _call(device, fn, *args):
     """fn(*args, the current stream of `device`) with `device` current, whichever is outside.  (The stream is asked for by its handle: the object that
     torch.cuda.current_stream() makes costs as much as the launch of a small kernel, 3 us.)"""
     i = device.index
-    if i == torch.cuda.current_device():
+    if i == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
@@ -353,13 +354,16 @@ def _token_strides(t, name):
         raise _L.WanHipError(f"{name} must be a CUDA(HIP) tensor -- libwanhip has no CPU path")
     if t.dtype != BF16:
         raise _L.WanHipError(f"{name} must be {BF16}, got {t.dtype}")
-    if t.dim() != 4 or t.shape[3] != 128:
-        raise _L.WanHipError(f"{name} must be [B, L, H, 128], got {list(t.shape)}")
-    B, L, H, _ = t.shape
-    if t.stride(3) != 1 or (H > 1 and t.stride(2) != 128):
+    shape = t.shape
+    if len(shape) != 4 or shape[3] != 128:
+        raise _L.WanHipError(f"{name} must be [B, L, H, 128], got {list(shape)}")
+    B, L, H, _ = shape
+    batch, row, head, one = t.stride()
+    if one != 1 or (H > 1 and head != 128):
         raise _L.WanHipError(f"{name}: the heads of a row must be contiguous")
-    row = t.stride(1) if L > 1 else H * 128
-    return row, (t.stride(0) if B > 1 else L * row)
+    if L <= 1:
+        row = H * 128
+    return row, (batch if B > 1 else L * row)
 
 
 def _lens(t, n, name, device):
@@ -451,9 +455,9 @@ def _mx_rows(x):
         raise _L.WanHipError("x must be a CUDA(HIP) tensor -- libwanhip has no CPU path")
     if x.dtype != BF16:
         raise _L.WanHipError(f"x must be {BF16}, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+    K = x.shape[-1] if x.dim() else 0
+    if K == 0 or K % 32:
         raise _L.WanHipError(f"the last dimension of x must be a positive multiple of 32, got {list(x.shape)}")
-    K = x.shape[-1]
     if x.is_contiguous():
         return x.numel() // K, K, K
     if x.dim() == 2 and x.stride(1) == 1:
@@ -475,11 +479,13 @@ def mxfp4_quantize(x):
 
 def _mx_operand(codes, scales, name):
     _req(codes, torch.uint8, name); _req(scales, torch.uint8, name + " scales")
-    if codes.dim() < 1 or codes.shape[-1] == 0 or codes.shape[-1] % 16:
-        raise _L.WanHipError(f"{name}: the last dimension must be a positive multiple of 16 bytes (32 values), got {list(codes.shape)}")
+    shape = codes.shape
+    row = shape[-1] if shape else 0
+    if row == 0 or row % 16:
+        raise _L.WanHipError(f"{name}: the last dimension must be a positive multiple of 16 bytes (32 values), got {list(shape)}")
     _same_device(codes, scales)
-    K = codes.shape[-1] * 2
-    M = codes.numel() // (K // 2)
+    K = row * 2
+    M = codes.numel() // row
     need = _L.load().wan_mxfp4_scale_bytes(M, K)
     if scales.numel() != need:
         raise _L.WanHipError(f"{name} scales must hold {need} bytes, got {scales.numel()}")
