@@ -129,7 +129,9 @@ def test_block_mean_of_a_slice_of_a_fused_projection(ops):
 # ---- select_blocks ---------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Bk,H,Hk,nq,nk,keep,lens", [(1, 1, 1, 1, 1, 1, 1, None), (1, 1, 2, 1, 3, 17, 5, None), (2, 2, 4, 2, 9, 65, 16, [4100, 130]), (2, 1, 3, 3, 5, 64, 64, None),
                                                        (1, 1, 1, 1, 70, 300, 37, None), (1, 1, 2, 2, 2, 30, 50, [0]), (2, 2, 1, 1, 4, 200, 1, [12800, 1]), (1, 1, 1, 1, 2, 1500, 600, None),
-                                                       (1, 1, 1, 1, 2, 5000, 700, [319999]), (1, 1, 2, 1, 3, 20000, 900, None), (1, 1, 1, 1, 70, 2049, 2048, None)])
+                                                       (1, 1, 1, 1, 2, 5000, 700, [319999]), (1, 1, 2, 1, 3, 20000, 900, None), (1, 1, 1, 1, 70, 2049, 2048, None), (2, 1, 3, 1, 17, 256, 30, [16300]), (1, 1, 2, 2, 33, 257, 256, None),
+                                                       (1, 1, 3, 3, 16, 640, 64, None), (2, 2, 2, 1, 31, 641, 70, [41000, 0]), (1, 1, 5, 1, 49, 1216, 148, [77800]), (1, 1, 2, 1, 20, 1217, 148, None),
+                                                       (3, 3, 1, 1, 15, 1180, 7, [1, 449, 75520])])
 def test_select_blocks(ops, B, Bk, H, Hk, nq, nk, keep, lens):
     g = gen(nk + keep)
     qm = torch.randn(B, H, nq, 128, generator=g, device="cuda")

@@ -44,7 +44,7 @@ def gemm(so, **kw):
     (mean, dict(x=None), "null"), (mean, dict(out=None), "null"), (mean, dict(L=0), "empty"), (mean, dict(block=0), "empty"), (mean, dict(B=0), "empty"), (mean, dict(row=504), "strides"),
     (mean, dict(row=516), "strides"), (mean, dict(batch=5121), "strides"), (mean, dict(x=ODD), "aligned"), (mean, dict(B=70000), "grid"),
     (select, dict(index=None), "null"), (select, dict(k=None), "null"), (select, dict(Bk=3), "Bk must divide"), (select, dict(Hk=3), "heads"), (select, dict(Hk=0), "heads"), (select, dict(keep=0), "empty"),
-    (select, dict(nk=0), "empty"), (select, dict(nk=20001, n=1 << 40), "20,000"), (select, dict(ws=None), "scratch"), (select, dict(n=2 * 4 * 3 * 5 * 8 - 1), "scratch"), (select, dict(ws=ODD), "scratch"),
+    (select, dict(nk=0), "empty"), (select, dict(nk=20001, n=1 << 40), "20,000"), (select, dict(nk=257, ws=None), "scratch"), (select, dict(nk=257, n=2 * 4 * 3 * 257 * 8 - 1), "scratch"), (select, dict(nk=257, ws=ODD, n=1 << 30), "scratch"),
     (select, dict(nq=1 << 30, n=1 << 60), "grid"),
     (attend, dict(q=None), "null"), (attend, dict(index=None), "null"), (attend, dict(Bk=4), "Bk must divide"), (attend, dict(Hk=3), "heads"), (attend, dict(Lk=0), "empty"), (attend, dict(keep=0), "empty"),
     (attend, dict(ldv=100), "ldv"), (attend, dict(ldv=64), "ldv"), (attend, dict(qr=504), "strides"), (attend, dict(kr=260), "strides"), (attend, dict(kb=3), "strides"), (attend, dict(vt=ODD), "aligned"),
@@ -82,6 +82,7 @@ def test_linear_entry_refuses():
 def test_scratch_and_scale_sizes():
     L = lib.load()
     assert L.wan_mxfp4_scale_bytes(1, 32) == 1024 and L.wan_mxfp4_scale_bytes(129, 257) == 4096 and L.wan_mxfp4_scale_bytes(0, 32) == 0 and L.wan_mxfp4_scale_bytes(75600, 13824) == 591 * 54 * 1024
+    assert L.wan_select_blocks_scratch_bytes(2, 4, 3, 256) == 0 and L.wan_select_blocks_scratch_bytes(2, 4, 3, 257) == 2 * 4 * 3 * 257 * 8   # (fewer stay in the LDS)
     assert L.wan_select_blocks_scratch_bytes(0, 1, 1, 1) == 0 and L.wan_select_blocks_scratch_bytes(1, 40, 591, 1182) >= 0
 
 

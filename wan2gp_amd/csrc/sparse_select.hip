@@ -70,46 +70,56 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
-// keys[row][j], on v_mfma_f64_16x16x4_f64: lane (n, g) supplies A[n][g] (query block n) and B[g][n] (key block n) of a step; register i holds D[4 i + g][n].  A
+// Scores on v_mfma_f64_16x16x4_f64: lane (n, g) supplies A[n][g] (query block n) and B[g][n] (key block n) of a step; register i holds D[4 i + g][n].  A
 // sum's order is free, so step 4 s + e takes column 16 s + 4 g + e: a load of four floats a lane is 64 consecutive bytes of each row (32 consecutive floats a
-// lane read every line of the L2 four times: 223 us).  One wave per 16 query blocks x `tiles` tiles of
-// 16 key blocks (even: eight, down to two where that leaves fewer than 2,048 waves: 24 heads x 13 x 512 take 5.0 us
-// with two, 14.1 with eight); the query block's 32 doubles stay in registers, and the four waves of a workgroup read the same keys.  Bound by the fp64 matrix rate (a step 64
-// cycles) and the conversions in front of it: 40 heads x 591 x 1,182 in 173 us, 41 TFLOP/s and 223 MB of scores written.
+// lane read every line of the L2 four times).  Two tiles of 16 key blocks at a time: two independent chains of products, and twice the loads in flight.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
+struct QueryMeans {
+  double a[32];
+};
+__device__ __forceinline__ QueryMeans load_queries(const float* qp) {   // (of the lane's row, from its column 4 g on)
+  QueryMeans q;
+#pragma unroll
+  for (int s = 0; s < 32; s += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(qp + 4 * s);
+    q.a[s] = v.x; q.a[s + 1] = v.y; q.a[s + 2] = v.z; q.a[s + 3] = v.w;
+  }
+  return q;
+}
+__device__ __forceinline__ void score_pair(const QueryMeans& q, const float* kp, int k0, int n, int nk, f64x4 (&acc)[2]) {
+  float4 v[2][8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const float* r = kp + (int64_t)min(k0 + 16 * u + n, nk - 1) * 128;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) v[u][s] = *reinterpret_cast<const float4*>(r + 16 * s);
+  }
+  acc[0] = acc[1] = f64x4{0., 0., 0., 0.};
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const float f[2][4] = {{v[0][s].x, v[0][s].y, v[0][s].z, v[0][s].w}, {v[1][s].x, v[1][s].y, v[1][s].z, v[1][s].w}};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(q.a[4 * s + e], (double)f[0][e], acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(q.a[4 * s + e], (double)f[1][e], acc[1], 0, 0, 0);
+    }
+  }
+}
+
+// More than 256 blocks of keys: the scores go to memory, keys[row][j].  One wave per 16 query blocks x `tiles` tiles of key blocks (even: eight, down to two where that leaves
+// fewer than 2,048 waves: 24 heads x 13 x 512 take 5.0 us with two, 14.1 with eight); the four waves of a workgroup read the same keys.  Bound by the fp64 matrix rate (a step
+// 64 cycles) and the conversions in front of it: 40 heads x 591 x 1,182 in 173 us, 41 TFLOP/s and 223 MB of scores written.
 __global__ __launch_bounds__(256) void block_score_kernel(const float* __restrict__ qm, const float* __restrict__ km, uint64_t* __restrict__ keys, int H, int Hk,
                                                          int Bk, int nq, int nk, int tiles) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int bh = blockIdx.z, b = bh / H, h = bh - b * H;
   const int q0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 16, k0 = blockIdx.x * (16 * tiles);
   if (q0 >= nq) return;
-  const float* qp = qm + ((int64_t)bh * nq + min(q0 + n, nq - 1)) * 128 + 4 * g;
+  const QueryMeans qs = load_queries(qm + ((int64_t)bh * nq + min(q0 + n, nq - 1)) * 128 + 4 * g);
   const float* kp = km + ((int64_t)(b % Bk) * Hk + h / (H / Hk)) * nk * 128 + 4 * g;
-  double a[32];
-#pragma unroll
-  for (int s = 0; s < 32; s += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(qp + 4 * s);
-    a[s] = v.x; a[s + 1] = v.y; a[s + 2] = v.z; a[s + 3] = v.w;
-  }
-  // two tiles at a time: two independent chains of products, and twice the loads in flight
   for (int t = 0; t < tiles && k0 + 16 * t < nk; t += 2) {
-    float4 v[2][8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float* r = kp + (int64_t)min(k0 + 16 * (t + u) + n, nk - 1) * 128;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) v[u][s] = *reinterpret_cast<const float4*>(r + 16 * s);
-    }
-    f64x4 acc[2] = {{0., 0., 0., 0.}, {0., 0., 0., 0.}};
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const float f[2][4] = {{v[0][s].x, v[0][s].y, v[0][s].z, v[0][s].w}, {v[1][s].x, v[1][s].y, v[1][s].z, v[1][s].w}};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * s + e], (double)f[0][e], acc[0], 0, 0, 0);
-        acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[4 * s + e], (double)f[1][e], acc[1], 0, 0, 0);
-      }
-    }
+    f64x4 acc[2];
+    score_pair(qs, kp, k0 + 16 * t, n, nk, acc);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -124,31 +134,15 @@ __global__ __launch_bounds__(256) void block_score_kernel(const float* __restric
 // Both kernels find the keep-th largest key bit by bit from the top (t: the largest value that at least `want` keys reach; they stop as soon as exactly that
 // many do), then emit what is above it and the first of what equals it, in ascending order.  A key 0 is none.
 
-// One wave per row, N keys a lane in registers, first over the keys' upper halves -- 20 of the mantissa's bits decide nearly every row.
-// Bound by the scores' bytes and the ballots: 23,640 rows of 1,182 in 60 us, 3.7 TB/s.  The whole choice took 236 us so and 390 us with the
-// search by a workgroup below; 33 against 59 us at 128 x 256, 609 against 937 us at 1,024 x 2,048.
-template <int N>
-__global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
-                                                               int* __restrict__ count, int H, int Bk, int nq, int nk, int keep, int64_t rows) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
+// A wave, N keys a lane in registers, first over the keys' upper halves -- 20 of the mantissa's bits decide nearly every row.
+template <int N, class F>
+__device__ __forceinline__ void select_row(F&& key, int n, int want, int* idx) {
   const int lane = threadIdx.x & 63;
-  const int b = (int)(r / ((int64_t)H * nq));
-  int n = nk;
-  if (k_lens != nullptr) n = min(nk, max(0, (int)(((int64_t)k_lens[b % Bk] + KEY_BLOCK - 1) / KEY_BLOCK)));
-  int* idx = index + r * keep;
-  const int want = min(keep, n);
-  if (lane == 0) count[r] = want;
-  for (int i = want + lane; i < keep; i += 64) idx[i] = -1;
-  if (want == n) {
-    for (int i = lane; i < n; i += 64) idx[i] = i;
-    return;
-  }
   uint32_t hi[N], lo[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int i = j * 64 + lane;
-    const uint64_t k = i < n ? keys[r * nk + i] : 0ull;
+    const uint64_t k = i < n ? key(i) : 0ull;
     hi[j] = (uint32_t)(k >> 32);
     lo[j] = (uint32_t)k;
   }
@@ -189,6 +183,65 @@ __global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* 
     out += __popcll(tk);
     room -= min(room, (int)__popcll(eqs));
   }
+}
+
+// count and what of the list does not depend on scores; true: the list is complete
+__device__ __forceinline__ bool open_row(int* idx, int* count, int n, int want, int keep) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) *count = want;
+  for (int i = want + lane; i < keep; i += 64) idx[i] = -1;
+  if (want < n) return false;
+  for (int i = lane; i < n; i += 64) idx[i] = i;
+  return true;
+}
+__device__ __forceinline__ int candidates(const int* k_lens, int b, int nk) {
+  return k_lens == nullptr ? nk : min(nk, max(0, (int)(((int64_t)k_lens[b] + KEY_BLOCK - 1) / KEY_BLOCK)));
+}
+
+// Up to 256 blocks of keys: scores and choice in one launch, the scores never leave the LDS.  Eight waves take the key tiles of 16 query blocks in turn, then two of their rows
+// each.  40 heads x 128 x 256: 22 us, in two launches 34.  (With more keys the two phases one behind the other leave too much idle: 13 x 1,182 takes 44 us so and 28 in two launches,
+// 591 x 1,182 271 and 235.)
+constexpr int CHOOSE_KEYS = 256;
+__global__ __launch_bounds__(512) void block_choose_kernel(const float* __restrict__ qm, const float* __restrict__ km, const int* __restrict__ k_lens, int* __restrict__ index,
+                                                          int* __restrict__ count, int H, int Hk, int Bk, int nq, int nk, int keep) {
+  __shared__ uint64_t row[16 * CHOOSE_KEYS];
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bh = blockIdx.y, b = bh / H, h = bh - b * H, q0 = blockIdx.x * 16;
+  const int have = candidates(k_lens, b % Bk, nk), want = min(keep, have);
+  if (want < have) {
+    const QueryMeans qs = load_queries(qm + ((int64_t)bh * nq + min(q0 + n, nq - 1)) * 128 + 4 * g);
+    const float* kp = km + ((int64_t)(b % Bk) * Hk + h / (H / Hk)) * nk * 128 + 4 * g;
+    const int k0 = wave * 32;
+    if (k0 < have) {
+      f64x4 acc[2];
+      score_pair(qs, kp, k0, n, nk, acc);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          row[(4 * i + g) * CHOOSE_KEYS + k0 + 16 * u + n] = order_key(acc[u][i]);   // (k0 + 31 < 256)
+    }
+  }
+  __syncthreads();
+  for (int r = wave; r < 16 && q0 + r < nq; r += 8) {
+    const int64_t at = (int64_t)bh * nq + q0 + r;
+    if (open_row(index + at * keep, count + at, have, want, keep)) continue;
+    const uint64_t* keys = row + r * CHOOSE_KEYS;
+    select_row<CHOOSE_KEYS / 64>([&](int i) { return keys[i]; }, have, want, index + at * keep);
+  }
+}
+
+// Up to 2,048: one wave per row, its keys from memory.  Bound by the ballots and the scores' bytes: 23,640 rows of 1,182 in 60 us.  The whole choice took 236 us so and 390 us with
+// the search by a workgroup below; 609 against 937 us at 1,024 x 2,048.
+template <int N>
+__global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
+                                                               int* __restrict__ count, int H, int Bk, int nq, int nk, int keep, int64_t rows) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int n = candidates(k_lens, (int)(r / ((int64_t)H * nq)) % Bk, nk), want = min(keep, n);
+  if (open_row(index + r * keep, count + r, n, want, keep)) return;
+  select_row<N>([&](int i) { return keys[r * nk + i]; }, n, want, index + r * keep);
 }
 
 // More than 2,048 blocks: one workgroup per row, the row's keys in LDS.  16 waves where the LDS has room for two rows or fewer (128 x 20,000 of 40 heads: 2.49 ms,
@@ -269,7 +322,7 @@ extern "C" int wan_block_mean(const wan_bf16* x, int64_t row_stride, int64_t bat
 }
 
 extern "C" int64_t wan_select_blocks_scratch_bytes(int B, int H, int64_t nq, int64_t nk) {
-  if (B < 1 || H < 1 || nq < 1 || nk < 1) return 0;
+  if (B < 1 || H < 1 || nq < 1 || nk <= CHOOSE_KEYS) return 0;   // (the scores stay in the LDS)
   return (int64_t)B * H * nq * nk * 8;
 }
 
@@ -281,26 +334,30 @@ extern "C" int wan_select_blocks(const float* q_mean, const float* k_mean, const
   WAN_REQUIRE(nq >= 1 && nk >= 1 && keep >= 1, "wan_select_blocks: empty problem (nq=%lld nk=%lld keep=%d)", (long long)nq, (long long)nk, keep);
   WAN_REQUIRE(nk <= 20000, "wan_select_blocks: %lld blocks of keys (at most 20,000: a row of scores has to fit the LDS)", (long long)nk);
   WAN_REQUIRE((int64_t)B * H < 65536 && (int64_t)B * H * nq < ((int64_t)1 << 31) && (nq + 63) / 64 < 65536, "wan_select_blocks: grid too large");
-  WAN_REQUIRE(scratch && scratch_bytes >= wan_select_blocks_scratch_bytes(B, H, nq, nk) && ((uintptr_t)scratch & 15) == 0,
-              "wan_select_blocks: needs 16-byte aligned scratch of %lld bytes", (long long)wan_select_blocks_scratch_bytes(B, H, nq, nk));
+  const int64_t need = wan_select_blocks_scratch_bytes(B, H, nq, nk);
+  WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_select_blocks: needs 16-byte aligned scratch of %lld bytes", (long long)need);
   WAN_REQUIRE((((uintptr_t)q_mean | (uintptr_t)k_mean) & 15) == 0, "wan_select_blocks: the means must be 16-byte aligned");
   hipStream_t st = as_stream(stream);
+  if (nk <= CHOOSE_KEYS) {
+    hipLaunchKernelGGL(block_choose_kernel, dim3((unsigned)((nq + 15) / 16), (unsigned)(B * H)), dim3(512), 0, st, q_mean, k_mean, k_lens, index, count, H, Hk, Bk, (int)nq, (int)nk, keep);
+    WAN_LAUNCH_CHECK();
+    return 0;
+  }
   uint64_t* keys = reinterpret_cast<uint64_t*>(scratch);
   int tiles = 8;
   while (tiles > 2 && (nk + 16 * tiles - 1) / (16 * tiles) * ((nq + 15) / 16) * B * H < 2048) tiles /= 2;
-  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 16 * tiles - 1) / (16 * tiles)), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean,
-                     keys, H, Hk, Bk, (int)nq, (int)nk, tiles);
+  hipLaunchKernelGGL(block_score_kernel, dim3((unsigned)((nk + 16 * tiles - 1) / (16 * tiles)), (unsigned)((nq + 63) / 64), (unsigned)(B * H)), dim3(256), 0, st, q_mean, k_mean, keys, H,
+                     Hk, Bk, (int)nq, (int)nk, tiles);
   WAN_LAUNCH_CHECK();
   const int64_t rows = (int64_t)B * H * nq;
   const dim3 grid((unsigned)((rows + 3) / 4)), wg(256);
 #define SELECT(N) hipLaunchKernelGGL(block_select_wave_kernel<N>, grid, wg, 0, st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep, rows)
-  if (nk <= 256) SELECT(4);
-  else if (nk <= 640) SELECT(10);
+  if (nk <= 640) SELECT(10);
   else if (nk <= 1216) SELECT(19);
   else if (nk <= 2048) SELECT(32);
+#undef SELECT
   else if (nk <= 6800) hipLaunchKernelGGL(block_select_kernel<4>, dim3((unsigned)rows), wg, (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
   else hipLaunchKernelGGL(block_select_kernel<16>, dim3((unsigned)rows), dim3(1024), (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
-#undef SELECT
   WAN_LAUNCH_CHECK();
   return 0;
 }

@@ -409,8 +409,8 @@ def select_blocks(q_mean, k_mean, keep, k_lens=None):
         return index, count
     lib = _L.load()
     need = int(lib.wan_select_blocks_scratch_bytes(B, H, nq, nk))
-    ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device)
-    _call(q_mean.device, lib.wan_select_blocks, q_mean.data_ptr(), k_mean.data_ptr(), _addr(k_lens), index.data_ptr(), count.data_ptr(), B, Bk, H, Hk, nq, nk, keep, ws.data_ptr(), need)
+    ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device) if need else None
+    _call(q_mean.device, lib.wan_select_blocks, q_mean.data_ptr(), k_mean.data_ptr(), _addr(k_lens), index.data_ptr(), count.data_ptr(), B, Bk, H, Hk, nq, nk, keep, _addr(ws), need)
     return index, count
 
 
