@@ -243,7 +243,8 @@ int wan_attention_sp_remote(const wan_bf16* q, const wan_bf16* k_all, const wan_
  * wan_select_blocks: q_mean [B, H, nq, 128], k_mean [Bk, Hk, nk, 128] -> index [B, H, nq, keep]: the blocks of keys with the `keep` largest
  *   products q_mean . k_mean (summed in 64 bits; equal ones: the lowest first; NaN above everything), ascending, -1 behind the last;
  *   count [B, H, nq]: how many there are.  Only the first ceil(k_lens[b] / 64) blocks are candidates (k_lens: device int32 [Bk] or NULL = all).
- *   Query batch b reads k batch b mod Bk, query head h k head h / (H / Hk).  nk <= 20,000.  scratch: wan_select_blocks_scratch_bytes(...).
+ *   Query batch b reads k batch b mod Bk, query head h k head h / (H / Hk).  nk <= 20,000.  scratch: wan_select_blocks_scratch_bytes(...),
+ *   NULL where that is 0 (up to 256 blocks of keys).
  * wan_sparse_attention: softmax(q k^T / sqrt(128)) v over the keys of the listed blocks that lie below k_lens[b].  q [B, Lq, H, 128],
  *   k [Bk, Lk, Hk, 128] (rows / batches q_row, q_batch, k_row, k_batch elements apart), vt [Bk, Hk * 128, ldv] as wan_attention takes it
  *   (columns past k_lens may hold anything), o [B, Lq, H, 128] contiguous (may be q, where q is contiguous).  index / count as
