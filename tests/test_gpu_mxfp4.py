@@ -250,6 +250,50 @@ def test_linears_on_streams_beside_each_other(ops):
         assert all(torch.equal(o, cases[i // 3][2]) for i, o in enumerate(per))
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 128, 5120), (1, 7, 32), (3, 1536, 13824), (16, 5120, 5120), (16, 1160, 1056), (17, 1160, 1056), (7, 257, 288), (15, 1000, 8960), (16, 640, 17000 // 32 * 32),
+                                   (16, 640, 20000), (2, 30720, 1536), (16, 700, 2560), (16, 700, 2592), (8, 12300, 4800), (9, 12300, 4800), (1, 640, 4480), (1, 640, 4512), (1, 12288, 64000)])
+def test_linear_of_few_rows(ops, M, N, K):
+    """Both sides of the limits of the kernel for up to 16 rows: every epilogue, strided rows, rows quantised inside and in front."""
+    g = gen(M * N + K)
+    wide = rows(g, M, K + 64)
+    x = wide[:, 32 : K + 32] if M > 1 else wide[:, 32 : K + 32].contiguous()
+    w = (torch.randn(N, K, generator=g, device="cuda") / math.sqrt(K)).to(BF)
+    xm, wm = ops.mxfp4_quantize(x), ops.mxfp4_quantize(w)
+    xd, wd = ops.mxfp4_dequantize(*xm).to(F64), ops.mxfp4_dequantize(*wm).to(F64)
+    bias = torch.randn(N, generator=g, device="cuda").to(BF)
+    y, err = linear_ref(xd, wd, bias)
+    got = ops.linear_mxfp4(x, *wm, bias)
+    close(got, y, err + 2.0 ** -8 * (y.abs() + err))
+    assert torch.equal(got, ops.linear_mxfp4(None, *wm, bias, x_mx=xm))
+    gelu = torch.nn.functional.gelu(y, approximate="tanh")
+    bound = 1.13 * err + 2.0 ** -18 * y.abs()
+    close(ops.linear_mxfp4(x, *wm, bias, epilogue=1), gelu, bound + 2.0 ** -8 * (gelu.abs() + bound))
+    r = torch.randn(M, N, generator=g, device="cuda").to(BF)
+    mod, e = torch.randn(6, N, generator=g, device="cuda").to(BF), torch.randn(M, 6, N, generator=g, device="cuda").to(BF)   # (a gate a row)
+    gate = mod[1].to(F64) + e[:, 1].to(F64)
+    out = r.to(F64) + y * gate
+    bound = err * gate.abs() + 2.0 ** -22 * (r.to(F64).abs() + (y * gate).abs())
+    inplace = r.clone()
+    close(ops.linear_mxfp4(x, *wm, bias, epilogue=2, residual=inplace, out=inplace, mod=mod, e=e, gate_idx=1), out, bound + 2.0 ** -8 * (out.abs() + bound))
+    vt = torch.full((N + 1, 64), 7.0, dtype=BF, device="cuda")
+    ops.linear_mxfp4(x, *wm, bias, epilogue=3, out=vt[:N], ldc=64)
+    close(vt[:N, :M], y.t(), (err + 2.0 ** -8 * (y.abs() + err)).t())
+    assert (vt[N:] == 7).all() and (vt[:, M:] == 7).all()
+
+
+def test_few_rows_with_nonfinite_blocks(ops):
+    """A row with an infinity or a NaN is NaN, its neighbours are not touched."""
+    g = gen(31)
+    x = rows(g, 5, 512)
+    x[1, 40], x[3, 511] = float("nan"), float("inf")
+    w = (torch.randn(300, 512, generator=g, device="cuda") / 20).to(BF)
+    wm = ops.mxfp4_quantize(w)
+    got = ops.linear_mxfp4(x, *wm)
+    assert torch.isnan(got[[1, 3]]).all()
+    x[[1, 3]] = 0
+    assert torch.equal(got[[0, 2, 4]], ops.linear_mxfp4(x, *wm)[[0, 2, 4]])
+
+
 def test_captured_linears_of_two_graphs(ops):
     g = gen(7)
     state = []

@@ -68,15 +68,16 @@ def test_quantiser_entries_refuse():
 
 def test_linear_entry_refuses():
     L = lib.load()
-    for kw, word in ((dict(x=None), "null"), (dict(W=None), "null"), (dict(M=0), "positive"), (dict(K=40), "multiple of 32"), (dict(n=100), "scratch"), (dict(ws=None), "scratch"), (dict(row=32), "row stride"),
+    for kw, word in ((dict(x=None), "null"), (dict(W=None), "null"), (dict(M=0), "positive"), (dict(K=40), "multiple of 32"), (dict(M=17, n=100), "scratch"), (dict(M=17, ws=None), "scratch"), (dict(row=32), "row stride"), (dict(M=17, row=68), "row stride"),
                      (dict(epi=2), "residual"), (dict(epi=7), "unknown epilogue"), (dict(ldc=63), "ldc"), (dict(C=ODD), "aligned"), (dict(x=ODD), "aligned")):
         a = dict(x=A, row=64, W=A, Ws=A, C=A, ldc=64, M=3, N=64, K=64, epi=0, ws=A, n=1 << 40) | kw
         refuse(L.wan_linear_mxfp4(a["x"], a["row"], a["W"], a["Ws"], None, a["C"], a["ldc"], a["M"], a["N"], a["K"], a["epi"], None, None, None, 0, -1, 1, a["ws"], a["n"], None), word)
-    need = L.wan_gemm_mxfp4_scratch_bytes(3, 64, 5120)
+    need = L.wan_gemm_mxfp4_scratch_bytes(17, 64, 5120)
     assert need > 0
-    refuse(gemm(L, K=5120, n=need - 1), "scratch")
-    refuse(gemm(L, K=5120, ws=None), "scratch")
-    assert L.wan_linear_mxfp4_scratch_bytes(3, 64, 5120) >= 3 * 2560 + 20 * 1024 + need and L.wan_gemm_mxfp4_scratch_bytes(4096, 5120, 5120) == 0
+    refuse(gemm(L, M=17, K=5120, n=need - 1), "scratch")
+    refuse(gemm(L, M=17, K=5120, ws=None), "scratch")
+    assert L.wan_linear_mxfp4_scratch_bytes(16, 64, 2560) == 0 and L.wan_gemm_mxfp4_scratch_bytes(16, 64, 2560) == 0   # (few rows stay in the LDS)
+    assert L.wan_linear_mxfp4_scratch_bytes(17, 64, 5120) >= 17 * 2560 + 20 * 1024 + need and L.wan_gemm_mxfp4_scratch_bytes(4096, 5120, 5120) == 0
 
 
 def test_scratch_and_scale_sizes():

@@ -257,6 +257,129 @@ __global__ __launch_bounds__(256) void mxg_join_kernel(MxGemm p, int parts, cons
     if (x + w < n) p.C[y * p.ldc + x + w] = mxg_finish<EPI>(p, o[w], y, x + w);
 }
 
+// ---- up to 16 rows: the weights straight from memory ------------------------------------------------------------------------------------
+// One workgroup per 128-row panel of the weights, wave t of each half of K its rows 8 n + t: a lane's 16 bytes of codes are one block, its 16 bytes of scales the eight waves' (byte t & 3 of
+// dwords t >> 2 and 2 + (t >> 2)).  The activations -- bf16 rows that are quantised here (X), or codes and scales -- lie in the LDS as a whole.  The weights of four
+// stages (8 KB a wave) are in flight while the four before are multiplied, the first ones in front of the quantisation.  Bound by the weights' bytes: 30,720 x 5,120 for one
+// row in 15.7 us, 5.3 TB/s.
+constexpr int MXR_ROWS = 16, MXR_LDS = 144 * 1024;
+struct MxRows {
+  const bf16_t* x;   // null: A, As
+  int64_t x_row;
+  const uint8_t *A, *As, *W, *Ws;
+  int64_t N;
+  int M;
+};
+__host__ __device__ constexpr int mxr_pitch(int K) { return K / 2 + 16; }         // (a row's 16 bytes more: the rows of a fragment read start at other banks)
+__host__ __device__ constexpr int mxr_scales(int K) { return (K / 32 + 15) & ~15; }
+
+typedef int mx_i8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ mx_i8 mx_wide(const mx_u4& v) { return mx_i8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }   // (of which a 4-bit operand reads the first four)
+
+template <int EPI>
+__global__ __launch_bounds__(1024) void gemm_mxfp4_rows_kernel(MxRows r, MxGemm p) {
+  extern __shared__ __attribute__((aligned(16))) char rows_lds[];   // codes [M][pitch], scale bytes [M][scales]
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int t = __builtin_amdgcn_readfirstlane((tid >> 6) & 7), half = __builtin_amdgcn_readfirstlane(tid >> 9);
+  const int K = p.K, kt = p.kt, blocks = K / 32, pitch = mxr_pitch(K), sp = mxr_scales(K);
+  uint8_t* codes = reinterpret_cast<uint8_t*>(rows_lds);
+  uint8_t* scales = codes + r.M * pitch;
+  const int64_t col = (int64_t)blockIdx.x * 128 + 8 * n + t;
+  const uint8_t* w = r.W + min(col, r.N - 1) * (K / 2) + 16 * g;                   // past the matrix: its last row again, never stored
+  const uint8_t* ws = r.Ws + (int64_t)blockIdx.x * kt * 1024 + lane * 16;
+  struct Batch {
+    mx_u4 c[4][2], s[4];
+  };
+  const int first = kt * half / 2, end = kt * (half + 1) / 2;
+  auto fetch = [&](Batch& b, int s0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i;
+      if (s < end) b.s[i] = *reinterpret_cast<const mx_u4*>(ws + (int64_t)s * 1024);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        b.c[i][ks] = mx_u4{0u, 0u, 0u, 0u};
+        if (s < end && 8 * s + 4 * ks + g < blocks) b.c[i][ks] = *reinterpret_cast<const mx_u4*>(w + s * 128 + ks * 64);
+      }
+    }
+  };
+  Batch cur, nxt;
+  fetch(cur, first);
+  for (int i = tid; i < r.M * blocks; i += 1024) {
+    const int m = i / blocks, j = i - m * blocks;
+    mx_u4 c;
+    uint32_t e;
+    if (r.x != nullptr) {
+      const bf16_t* x = r.x + m * r.x_row + j * 32;
+      uint32_t a = 0;
+      float f[32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) unpack8(*reinterpret_cast<const uint4*>(x + 8 * q), f + 8 * q);
+#pragma unroll
+      for (int q = 0; q < 32; ++q) a = max(a, __float_as_uint(f[q]) & 0x7fffffffu);
+      e = mxfp4_scale(a);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t v = mxfp4_encode8(f + 8 * q, e);
+        c[q] = v;
+      }
+    } else {
+      c = *reinterpret_cast<const mx_u4*>(r.A + (int64_t)m * (K / 2) + j * 16);
+      e = r.As[(j >> 3) * 1024 + (j & 3) * 256 + (m >> 3) * 16 + ((j >> 2) & 1) * 8 + (m & 7)];
+    }
+    *reinterpret_cast<mx_u4*>(codes + m * pitch + j * 16) = c;
+    scales[m * sp + j] = (uint8_t)e;
+  }
+  __syncthreads();
+  const int m = min(n, r.M - 1);   // (rows past the last: that one again, never stored)
+  const uint8_t* xc = codes + m * pitch + 16 * g;
+  const uint8_t* xs = scales + m * sp + g;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int sh = 8 * (t & 3);
+  const bool upper = t >= 4;
+  for (int s0 = first; s0 < end; s0 += 4) {
+    if (s0 + 4 < end) fetch(nxt, s0 + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i;
+      if (s >= end) break;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const int j = 8 * s + 4 * ks;
+        const bool in = j + g < blocks;
+        mx_u4 a = mx_u4{0u, 0u, 0u, 0u};
+        uint32_t sa = 0;
+        if (in) {
+          a = *reinterpret_cast<const mx_u4*>(xc + j * 16);
+          sa = xs[j];
+        }
+        const uint32_t word = upper ? cur.s[i][2 * ks + 1] : cur.s[i][2 * ks];
+        const uint32_t sw = in ? word >> sh : 0u;
+        // (the builtin: one chain of products, where hipcc's own wait states between them cost nothing)
+        if (EPI == WAN_EPI_TRANSPOSED) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(cur.c[i][ks]), mx_wide(a), acc, 4, 4, 0, (int)sw, 0, (int)sa);
+        else acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(a), mx_wide(cur.c[i][ks]), acc, 4, 4, 0, (int)sa, 0, (int)sw);
+      }
+    }
+    cur = nxt;
+  }
+  __syncthreads();   // (the codes are read)
+  f32x4* sums = reinterpret_cast<f32x4*>(rows_lds);
+  if (half == 1) sums[tid - 512] = acc;
+  __syncthreads();
+  if (half == 1) return;
+  acc += sums[tid];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (EPI == WAN_EPI_TRANSPOSED) {   // register i: weight row 8 (4 g + i) + t, token n
+      const int64_t y = (int64_t)blockIdx.x * 128 + 8 * (4 * g + i) + t;
+      if (y < r.N && n < r.M) p.C[y * p.ldc + n] = mxg_finish<EPI>(p, acc[i], y, n);
+    } else {
+      const int y = 4 * g + i;
+      if (y < r.M && col < r.N) p.C[y * p.ldc + col] = mxg_finish<EPI>(p, acc[i], y, col);
+    }
+  }
+}
+
 // Which kernel, and in how many parts along K: 0 = the 256 x 256 tiles of gemm_mxfp4m.hip, n = 128 x 128 tiles in n parts.  The least of what the
 // three were measured to take, in us: a round of up to 256 big tiles 8.5 + 1.2 a stage, of small ones 5.5 + 0.52 a stage, a join 5 and the partial
 // sums' bytes.  Both sides, M x N x K: 512 x 5,120 x 5,120 (40 big tiles) 29.3 big, 15.8 small; 1,024 x 5,120 x 13,824 (80) 68.5 and 62.2;
@@ -287,12 +410,35 @@ int mxg_launch(const MxGemm& p, int parts, float* scratch, hipStream_t st) {
   return 0;
 }
 
+// Whether a problem of few rows takes that kernel.  A workgroup streams its panel at the 30 GB/s that one CU gets, so few panels of long rows are better cut along K, the more so the
+// more rows each workgroup has to quantise.  In us with the quantisation, this kernel and the others, M x N x K: 1 x 1,536 x 1,536 5.4 and 9.1; 16 x 1,536 x 1,536 7.6 and 9.6;
+// 1 x 5,120 x 5,120 13.0 and 12.2; 16 x 5,120 x 5,120 16.8 and 13.8; 1 x 5,120 x 13,824 30.9 and 17.0.  With panels for most CUs: 1 x 30,720 x 5,120 15.7 and 19.3;
+// 4 x 13,824 x 5,120 15.5 and 16.6; 16 x 13,824 x 5,120 18.2 and 17.2.
+bool mxr_fits(int64_t M, int64_t N, int K) {
+  if (M > MXR_ROWS || M * (mxr_pitch(K) + mxr_scales(K)) > MXR_LDS) return false;
+  return K <= 4608 - 128 * M || (M <= 8 && N >= 96 * 128);
+}
+
+int mxr_launch(const bf16_t* x, int64_t x_row, const uint8_t* A, const uint8_t* As, const uint8_t* W, const uint8_t* Ws, int64_t M, int64_t N, const MxGemm& p, int epilogue, hipStream_t st) {
+  const MxRows r = {x, x_row, A, As, W, Ws, N, (int)M};
+  const dim3 grid((unsigned)((N + 127) / 128)), wg(1024);
+  const unsigned need = (unsigned)(M * (mxr_pitch(p.K) + mxr_scales(p.K))), lds = need > 8192 ? need : 8192;   // (the second half's sums: 8 KB)
+  switch (epilogue) {
+    case WAN_EPI_NONE: hipLaunchKernelGGL(gemm_mxfp4_rows_kernel<WAN_EPI_NONE>, grid, wg, lds, st, r, p); break;
+    case WAN_EPI_GELU_TANH: hipLaunchKernelGGL(gemm_mxfp4_rows_kernel<WAN_EPI_GELU_TANH>, grid, wg, lds, st, r, p); break;
+    case WAN_EPI_GATE_RES: hipLaunchKernelGGL(gemm_mxfp4_rows_kernel<WAN_EPI_GATE_RES>, grid, wg, lds, st, r, p); break;
+    default: hipLaunchKernelGGL(gemm_mxfp4_rows_kernel<WAN_EPI_TRANSPOSED>, grid, wg, lds, st, r, p); break;
+  }
+  WAN_LAUNCH_CHECK();
+  return 0;
+}
+
 }  // namespace
 
 int wan_gemm_mxfp4m_try(const MxGemm& p, int epilogue, hipStream_t st);   // gemm_mxfp4m.hip
 
 extern "C" int64_t wan_gemm_mxfp4_scratch_bytes(int64_t M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1) return 0;
+  if (M < 1 || N < 1 || K < 1 || mxr_fits(M, N, K)) return 0;
   const int parts = mxg_plan(M, N, (K + 255) / 256);
   return parts <= 1 ? 0 : (int64_t)parts * M * N * 4;
 }
@@ -324,6 +470,7 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
   hipStream_t st = as_stream(stream);
   const MxGemm p = {tr ? W : A, tr ? w_scales : a_scales, tr ? A : W, tr ? a_scales : w_scales, tr ? N : M, tr ? M : N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx,
                     rows_per_batch > 0 ? rows_per_batch : 1};
+  if (mxr_fits(M, N, K)) return mxr_launch(nullptr, 0, A, a_scales, W, w_scales, M, N, p, epilogue, st);
   const int plan = mxg_plan(M, N, p.kt);
   if (plan == 0) {
     const int rc = wan_gemm_mxfp4m_try(p, epilogue, st);
@@ -342,13 +489,23 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
 static int64_t mx_linear_codes(int64_t M, int K) { return (M * (K / 2) + 255) / 256 * 256; }
 
 extern "C" int64_t wan_linear_mxfp4_scratch_bytes(int64_t M, int N, int K) {
-  if (M < 1 || N < 1 || K < 32 || K % 32 != 0) return 0;
+  if (M < 1 || N < 1 || K < 32 || K % 32 != 0 || mxr_fits(M, N, K)) return 0;
   return mx_linear_codes(M, K) + wan_mxfp4_scale_bytes(M, K) + wan_gemm_mxfp4_scratch_bytes(M, N, K);
 }
 
 extern "C" int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue,
                                 const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes, void* stream) {
   WAN_REQUIRE(M >= 1 && N >= 1 && K >= 32 && K % 32 == 0, "wan_linear_mxfp4: M=%lld and N=%d must be positive, K=%d a positive multiple of 32", (long long)M, N, K);
+  if (mxr_fits(M, N, K)) {   // nothing of the quantised rows leaves the kernel
+    WAN_REQUIRE(x != nullptr, "wan_linear_mxfp4: null pointer");
+    WAN_REQUIRE(x_row >= K && x_row % 8 == 0, "wan_linear_mxfp4: the row stride %lld must be a multiple of 8 elements, at least K", (long long)x_row);
+    WAN_REQUIRE(((uintptr_t)x & 15) == 0, "wan_linear_mxfp4: pointers must be 16-byte aligned");
+    const uint8_t* some = reinterpret_cast<const uint8_t*>(x);
+    const int rc = mx_gemm_check(some, some, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
+    if (rc != 0) return rc;
+    const MxGemm p = {nullptr, nullptr, nullptr, nullptr, M, N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx, rows_per_batch > 0 ? rows_per_batch : 1};
+    return mxr_launch(x, x_row, nullptr, nullptr, W, w_scales, M, N, p, epilogue, as_stream(stream));
+  }
   const int64_t need = wan_linear_mxfp4_scratch_bytes(M, N, K);
   WAN_REQUIRE(scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0, "wan_linear_mxfp4: needs 16-byte aligned scratch of %lld bytes", (long long)need);
   uint8_t* codes = reinterpret_cast<uint8_t*>(scratch);
