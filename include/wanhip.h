@@ -169,7 +169,7 @@ int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, 
                    const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes,
                    void* stream);
 /* wan_mxfp4_quantize of x [M, K] bf16 (rows x_row elements apart) into the scratch, then wan_gemm_mxfp4: one call for a Linear whose
- * quantised input nobody else reads. */
+ * quantised input nobody else reads.  C must not overlap x (it may be R). */
 int64_t wan_linear_mxfp4_scratch_bytes(int64_t M, int N, int K);
 int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C,
                      int64_t ldc, int64_t M, int N, int K, int epilogue, const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e,

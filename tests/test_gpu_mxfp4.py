@@ -281,6 +281,21 @@ def test_linear_of_few_rows(ops, M, N, K):
     assert (vt[N:] == 7).all() and (vt[:, M:] == 7).all()
 
 
+def test_output_over_the_input_is_refused(ops):
+    from wan2gp_amd.lib import WanHipError
+    g = gen(32)
+    w = ops.mxfp4_quantize((torch.randn(512, 512, generator=g, device="cuda") / 22).to(BF))
+    for M in (3, 40):
+        buf = rows(g, 2 * M, 512)
+        x = buf[:M]
+        ref = ops.linear_mxfp4(x, *w)
+        with pytest.raises(WanHipError, match="overlap"):
+            ops.linear_mxfp4(x, *w, out=x)
+        with pytest.raises(WanHipError, match="overlap"):
+            ops.linear_mxfp4(x, *w, out=buf[1 : M + 1])
+        assert torch.equal(ops.linear_mxfp4(x, *w, out=buf[M:]), ref) and torch.equal(buf[M:], ref)
+
+
 def test_few_rows_with_nonfinite_blocks(ops):
     """A row with an infinity or a NaN is NaN, its neighbours are not touched."""
     g = gen(31)

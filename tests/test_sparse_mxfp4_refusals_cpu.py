@@ -72,6 +72,13 @@ def test_linear_entry_refuses():
                      (dict(epi=2), "residual"), (dict(epi=7), "unknown epilogue"), (dict(ldc=63), "ldc"), (dict(C=ODD), "aligned"), (dict(x=ODD), "aligned")):
         a = dict(x=A, row=64, W=A, Ws=A, C=A, ldc=64, M=3, N=64, K=64, epi=0, ws=A, n=1 << 40) | kw
         refuse(L.wan_linear_mxfp4(a["x"], a["row"], a["W"], a["Ws"], None, a["C"], a["ldc"], a["M"], a["N"], a["K"], a["epi"], None, None, None, 0, -1, 1, a["ws"], a["n"], None), word)
+    B = 1 << 24                                                        # (addresses alone are compared; every call here is refused)
+    for kw in (dict(x=B, C=B), dict(x=B, C=B + 128), dict(x=B, C=B - 16), dict(x=B, C=B + 16, M=200), dict(x=B, C=B + 64 * 2, row=128, ldc=96, M=200), dict(x=B, C=B + 256, epi=3, row=1024),
+               dict(x=B, C=B + 96, row=128, ldc=128)):
+        a = dict(x=A, row=64, W=A, Ws=A, C=A, ldc=64, M=3, N=64, K=64, epi=0, ws=A, n=1 << 40) | kw
+        if a["epi"] == 3:
+            a["ldc"] = 64
+        refuse(L.wan_linear_mxfp4(a["x"], a["row"], a["W"], a["Ws"], None, a["C"], a["ldc"], a["M"], a["N"], a["K"], a["epi"], None, None, None, 0, -1, 1, a["ws"], a["n"], None), "overlap")
     need = L.wan_gemm_mxfp4_scratch_bytes(17, 64, 5120)
     assert need > 0
     refuse(gemm(L, M=17, K=5120, n=need - 1), "scratch")

@@ -485,6 +485,16 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
   }
 }
 
+// Whether the output shares memory with x: workgroups may read x while others already write.  (Rows side by side in one buffer share a range, but no element.)
+static bool mx_overlaps(const wan_bf16* x, int64_t x_row, const wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue) {
+  const bool tr = epilogue == WAN_EPI_TRANSPOSED;
+  const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((M - 1) * x_row + K) * 2, c0 = (uintptr_t)C, c1 = c0 + ((tr ? N - 1 : M - 1) * ldc + (tr ? M : N)) * 2;
+  if (x1 <= c0 || c1 <= x0) return false;
+  if (tr || x_row != ldc || M == 1) return true;
+  const int64_t d = ((int64_t)(c0 / 2) - (int64_t)(x0 / 2)) % ldc, at = d < 0 ? d + ldc : d;   // C's first column, counted from x's
+  return !(at >= K && at + N <= ldc);
+}
+
 // the quantised rows and their scales in front of the product's own scratch
 static int64_t mx_linear_codes(int64_t M, int K) { return (M * (K / 2) + 255) / 256 * 256; }
 
@@ -496,13 +506,14 @@ extern "C" int64_t wan_linear_mxfp4_scratch_bytes(int64_t M, int N, int K) {
 extern "C" int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue,
                                 const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes, void* stream) {
   WAN_REQUIRE(M >= 1 && N >= 1 && K >= 32 && K % 32 == 0, "wan_linear_mxfp4: M=%lld and N=%d must be positive, K=%d a positive multiple of 32", (long long)M, N, K);
+  WAN_REQUIRE(x != nullptr, "wan_linear_mxfp4: null pointer");
+  WAN_REQUIRE(x_row >= K && x_row % 8 == 0, "wan_linear_mxfp4: the row stride %lld must be a multiple of 8 elements, at least K", (long long)x_row);
+  WAN_REQUIRE(((uintptr_t)x & 15) == 0, "wan_linear_mxfp4: pointers must be 16-byte aligned");
   if (mxr_fits(M, N, K)) {   // nothing of the quantised rows leaves the kernel
-    WAN_REQUIRE(x != nullptr, "wan_linear_mxfp4: null pointer");
-    WAN_REQUIRE(x_row >= K && x_row % 8 == 0, "wan_linear_mxfp4: the row stride %lld must be a multiple of 8 elements, at least K", (long long)x_row);
-    WAN_REQUIRE(((uintptr_t)x & 15) == 0, "wan_linear_mxfp4: pointers must be 16-byte aligned");
     const uint8_t* some = reinterpret_cast<const uint8_t*>(x);
     const int rc = mx_gemm_check(some, some, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
     if (rc != 0) return rc;
+    WAN_REQUIRE(!mx_overlaps(x, x_row, C, ldc, M, N, K, epilogue), "wan_linear_mxfp4: the output must not overlap x");
     const MxGemm p = {nullptr, nullptr, nullptr, nullptr, M, N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx, rows_per_batch > 0 ? rows_per_batch : 1};
     return mxr_launch(x, x_row, nullptr, nullptr, W, w_scales, M, N, p, epilogue, as_stream(stream));
   }
@@ -514,6 +525,7 @@ extern "C" int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t*
   // (the product's arguments are checked by a call that may refuse them: in front of the first launch)
   const int rc = mx_gemm_check(codes, scales, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
   if (rc != 0) return rc;
+  WAN_REQUIRE(!mx_overlaps(x, x_row, C, ldc, M, N, K, epilogue), "wan_linear_mxfp4: the output must not overlap x");
   const int rq = wan_mxfp4_quantize(x, x_row, codes, scales, M, K, stream);
   if (rq != 0) return rq;
   return wan_gemm_mxfp4(codes, scales, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch, rest, scratch_bytes - (rest - codes), stream);

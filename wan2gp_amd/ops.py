@@ -504,7 +504,8 @@ def mxfp4_dequantize(codes, scales):
 def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, residual=None, mod=None, e=None, gate_idx=-1, out=None, ldc=None,
                  x_mx=None):
     """nn.Linear on MXFP4 operands with an optional fused epilogue (linear's): x [..., K] bf16 is quantised (or pass x_mx = mxfp4_quantize(x) to share
-    it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight)."""
+    it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight).  out may be the
+    residual, not x."""
     for t, n in ((bias, "bias"), (residual, "residual"), (mod, "mod"), (e, "e"), (out, "out")):
         _req(t, BF16, n)
     if weight_codes.dim() != 2:
