@@ -247,7 +247,7 @@ int wan_attention_sp_remote(const wan_bf16* q, const wan_bf16* k_all, const wan_
  *   NULL where that is 0 (up to 256 blocks of keys).
  * wan_sparse_attention: softmax(q k^T / sqrt(128)) v over the keys of the listed blocks that lie below k_lens[b].  q [B, Lq, H, 128],
  *   k [Bk, Lk, Hk, 128] (rows / batches q_row, q_batch, k_row, k_batch elements apart), vt [Bk, Hk * 128, ldv] as wan_attention takes it
- *   (columns past k_lens may hold anything), o [B, Lq, H, 128] contiguous (may be q, where q is contiguous).  index / count as
+ *   (columns past k_lens may hold anything), o [B, Lq, H, 128] contiguous (may be q, where q is contiguous; overlaps nothing else).  index / count as
  *   wan_select_blocks leaves them, in any order; entries outside [0, ceil(k_lens / 64)) are skipped, a block listed twice counts twice;
  *   count NULL = all `keep` entries.  A query without a key gets zeros.  q_prescaled: q already holds q * wan_attention_qscale().
  *   scratch: wan_sparse_attention_scratch_bytes(...) bytes of device memory, 16-byte aligned (NULL where that is 0); a call overwrites it,

@@ -313,6 +313,23 @@ def test_more_lists_than_run_at_a_time(ops, B, Bk, H, Hk, Lq, Lk, keep, lens):
     assert ops.sparse_attention(q, k, vt, index, count, k_lens=lens_of(lens), out=q) is q and torch.equal(q, got)
 
 
+def test_output_over_an_input_is_refused(ops):
+    from wan2gp_amd.lib import WanHipError
+    g = gen(41)
+    for L in (12, 200):
+        both = rnd(g, 2, 1, L, 2, 128)
+        q, k, v = both[0], both[1], rnd(g, 1, L, 2, 128)
+        vt, index = vt_of(v), torch.zeros(1, 2, (L + 127) // 128, 1, dtype=torch.int32, device="cuda")
+        ref = ops.sparse_attention(q, k, vt, index)
+        for out in (k, both.view(-1)[256 : 256 + q.numel()].view_as(q), vt.view(-1)[: q.numel()].view_as(q)):
+            with pytest.raises(WanHipError, match="overlap"):
+                ops.sparse_attention(q, k, vt, index, out=out)
+        fused = rnd(g, 1, L, 2, 2, 128)                                          # a strided q, and an output over its memory
+        with pytest.raises(WanHipError, match="overlap"):
+            ops.sparse_attention(fused[:, :, 0], k, vt, index, out=fused.view(-1)[: q.numel()].view_as(q))
+        assert ops.sparse_attention(q, k, vt, index, out=q) is q and torch.equal(q, ref)
+
+
 # ---- up to 16 queries: a kernel of their own ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Bk,H,Hk,Lq,Lk,keep,lens", [(1, 1, 1, 1, 1, 1, 1, None), (2, 1, 6, 2, 2, 65, 3, None), (2, 2, 5, 1, 15, 2000, 31, [2000, 63]), (1, 1, 40, 8, 16, 9000, 141, [8999]),
                                                        (1, 1, 40, 8, 17, 9000, 141, [8999]), (3, 3, 400, 4, 1, 640, 9, [1, 64, 640]), (1, 1, 1, 1, 1, 75600, 1182, None),
@@ -429,6 +446,11 @@ def test_pay_sparse_attention(ops):
     two = ops.pay_sparse_attention([q, k[:1].repeat(2, 1, 1, 1), v[:1].repeat(2, 1, 1, 1)], 3)
     assert torch.equal(one, two)
     assert (ops.pay_sparse_attention([q, k[:, :0], v[:, :0]], 3) == 0).all()
+    same = ops.pay_sparse_attention([q, q.clone(), v], 3)                        # one tensor as q and k: its storage is not reused
+    keep = q.clone()
+    assert torch.equal(ops.pay_sparse_attention([q, q, v], 3, recycle_q=True), same) and torch.equal(q, keep)
+    got = ops.pay_sparse_attention([q, k, v], 3, recycle_q=True)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, ops.pay_sparse_attention([keep, k, v], 3))
 
 
 def test_captured_and_replayed_beside_another_graph(ops):

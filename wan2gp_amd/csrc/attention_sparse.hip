@@ -695,6 +695,11 @@ SparsePlan sparse_plan(int64_t Lq, int64_t lists, int keep) {
 
 }  // namespace
 
+static bool sp_shares(const wan_bf16* o, int64_t o_elements, const wan_bf16* t, int64_t t_elements) {
+  const uintptr_t a = (uintptr_t)o, b = (uintptr_t)t;
+  return a < b + t_elements * 2 && b < a + o_elements * 2;
+}
+
 extern "C" int64_t wan_sparse_attention_scratch_bytes(int B, int64_t Lq, int H, int keep) {
   if (B < 1 || Lq < 1 || H < 1 || keep < 1) return 0;
   const int64_t lists = (Lq + Q_BLOCK - 1) / Q_BLOCK * H * B;
@@ -721,6 +726,12 @@ extern "C" int wan_sparse_attention(const wan_bf16* q, int64_t q_row, int64_t q_
   const SparsePlan pl = sparse_plan(Lq, lists, keep);
   const int64_t need = wan_sparse_attention_scratch_bytes(B, Lq, H, keep);
   WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_sparse_attention: needs 16-byte aligned scratch of %lld bytes", (long long)need);
+  // one workgroup's output would be another's input (q itself is read by the workgroup alone that writes its place)
+  const int64_t on = (int64_t)B * Lq * H * 128;
+  WAN_REQUIRE(!sp_shares(o, on, k, (Bk - 1) * k_batch + (Lk - 1) * k_row + Hk * 128) && !sp_shares(o, on, vt, (int64_t)Bk * Hk * 128 * ldv),
+              "wan_sparse_attention: the output must not overlap k or vt");
+  WAN_REQUIRE(!sp_shares(o, on, q, (B - 1) * q_batch + (Lq - 1) * q_row + H * 128) || (o == q && (Lq == 1 || q_row == (int64_t)H * 128) && (B == 1 || q_batch == Lq * H * 128)),
+              "wan_sparse_attention: an output that overlaps q must be q, contiguous");
   hipStream_t st = as_stream(stream);
   const SparseArgs a = {q, k, vt, o, q_row, q_batch, k_row, k_batch, ldv, Lq, Lk, index, count, k_lens, B, Bk, H, Hk, (int)nq, keep, q_prescaled, pl.parts, (int)pl.whole, Lq <= FEW ? FEW : Q_BLOCK, reinterpret_cast<float*>(scratch)};
   const unsigned wgs = (unsigned)(pl.whole + pl.cut * pl.parts);

@@ -591,7 +591,8 @@ def pay_sparse_attention(qkv_list, keep, k_lens=None, recycle_q=False):
     if k.shape[1] == 0:
         return torch.zeros(q.shape, dtype=out_dtype, device=q.device)
     index, count = select_blocks(block_mean(q, 128), block_mean(k, 64, k_lens), keep, k_lens)
-    o = sparse_attention(q, k, transpose_v(v), index, count, k_lens=k_lens, out=q if (recycle_q and out_dtype == BF16 and q.is_contiguous()) else None)
+    own = q.is_contiguous() and q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr()
+    o = sparse_attention(q, k, transpose_v(v), index, count, k_lens=k_lens, out=q if (recycle_q and out_dtype == BF16 and own) else None)
     return o.type(out_dtype)
 
 
