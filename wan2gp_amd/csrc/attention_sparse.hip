@@ -674,10 +674,11 @@ __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs)
   *reinterpret_cast<uint32_t*>(p.o + ((int64_t)b * p.Lq + r) * p.H * 128 + (int64_t)h * 128 + 2 * lane) = cvt_pk(s0 * inv, s1 * inv);
 }
 
-// How a launch's lists are cut.  Up to 16 queries: one workgroup for every four blocks of a list, up to 1,024 in all.  Else 512 workgroups run at a time: what is
-// left of the lists behind whole rounds of 512 is cut into as many shares as fill a round, none shorter than two blocks.  (More shares than that cost more in partial
-// sums than they gain: 312 lists of 48 blocks 109 us whole, 137 in two shares each.)  516 lists of 64 blocks take 150 us so and 221 uncut, 612 lists 173 and 223, 756 lists
-// 206 and 225; 156 lists of 48 blocks in three shares 56, in two 61.
+// How a launch's lists are cut.  Up to 16 queries: one workgroup for every four blocks of a list, up to 1,024 in all.  Else 512 workgroups run at a time, and what is left
+// of the lists behind whole rounds of 512 is cut into the number of shares that takes the least time: what was measured is 1.4 us a block, and for shares 7 us for the join and
+// 0.28 ns for each of a list's rows and shares (its partial sums are written and read), while all of them run at a time.  Lists x blocks, in us whole and in shares:
+// 12 x 100 (64 queries each) 150, in 16 shares 32.8; 64 x 140 209, in 8 60.8, in 4 74; 96 x 32 60.5, in 4 41.6; 96 x 8 24.0, in 2 29.4; 36 x 4 15.7, in 2 17.6;
+// 312 x 48 109, in 2 137; 516 x 64 221, the last four in shares 150; 756 x 64 225 and 206.
 struct SparsePlan {
   int64_t whole, cut;
   int parts;
@@ -685,10 +686,19 @@ struct SparsePlan {
 SparsePlan sparse_plan(int64_t Lq, int64_t lists, int keep) {
   const bool few = Lq <= FEW;
   const int64_t whole = few ? 0 : lists / 512 * 512, cut = lists - whole;
-  int64_t n = cut > 0 ? (few ? 1024 : 512) / cut : 0;
-  const int64_t shares = few ? (keep + 3) / 4 : keep / 2, most = few ? 64 : 32;
-  if (n > shares) n = shares;
-  if (n > most) n = most;
+  int64_t n = 1;
+  if (few) {
+    n = 1024 / cut;
+    if (n > (keep + 3) / 4) n = (keep + 3) / 4;
+    if (n > 64) n = 64;
+  } else if (cut > 0) {
+    const double rows = (double)(cut * (Lq < Q_BLOCK ? Lq : Q_BLOCK));
+    double best = 1.4 * keep;
+    for (int k = 2; k <= 32 && k <= keep && k * cut <= 512; ++k) {
+      const double t = 1.4 * ((keep + k - 1) / k) + 7.0 + 0.00028 * rows * k;
+      if (t < best) { best = t; n = k; }
+    }
+  }
   if (n < 2) return {lists, 0, 1};
   return {whole, cut, (int)n};
 }

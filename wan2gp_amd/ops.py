@@ -427,15 +427,17 @@ def sparse_attention(q, k, vt, block_index, block_count=None, k_lens=None, out=N
     _same_device(q, k, vt, block_index, block_count, out)
     _lens(k_lens, Bk, "k_lens", q.device)
     nq = (Lq + 127) // 128
-    if block_index.dim() != 4 or tuple(block_index.shape[:3]) != (B, H, nq):
+    listed = block_index.shape
+    if len(listed) != 4 or listed[0] != B or listed[1] != H or listed[2] != nq:
         raise _L.WanHipError(f"block_index must be [{B}, {H}, {nq}, keep], got {list(block_index.shape)}")
-    if block_count is not None and tuple(block_count.shape) != (B, H, nq):
+    if block_count is not None and block_count.shape != listed[:3]:
         raise _L.WanHipError(f"block_count must be [{B}, {H}, {nq}], got {list(block_count.shape)}")
-    if vt.dim() != 3 or vt.shape[0] != Bk or vt.shape[1] != Hk * 128:
-        raise _L.WanHipError(f"vt must be [{Bk}, {Hk * 128}, ldv], got {list(vt.shape)}")
+    rows = vt.shape
+    if len(rows) != 3 or rows[0] != Bk or rows[1] != Hk * 128:
+        raise _L.WanHipError(f"vt must be [{Bk}, {Hk * 128}, ldv], got {list(rows)}")
     if out is not None and out.shape != q.shape:
         raise _L.WanHipError(f"out must be {list(q.shape)}, got {list(out.shape)}")
-    keep, ldv = block_index.shape[3], vt.shape[2]
+    keep, ldv = listed[3], rows[2]
     out = torch.empty(B, Lq, H, 128, dtype=BF16, device=q.device) if out is None else out
     if Lq == 0 or B == 0:
         return out
