@@ -26,8 +26,9 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
 //   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
 //     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
-// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 12.4 ms, 1.18 PFLOP/s, the matrix pipe busy for 60 % of the cycles at 1.9 GHz, the waves
-// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 733 us.
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 11.8 ms, 1.24 PFLOP/s, the matrix pipe busy for about 63 % of the cycles at 1.9 GHz, the waves
+// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 682 us.  (The queries' sixteen loads
+// one behind the other in front of the first tile cost 5 % of that.)
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
 // MFMA 0); a score is multiplied in the odd gap in front of its exp2, a pair packed in the odd gap behind its second, fragments summed by one MFMA more behind
 // the last product of each; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
@@ -343,10 +344,22 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   const int bk = uni(b % p.Bk), hk = uni(h / (p.H / p.Hk));
 
   typedef const __attribute__((address_space(4))) int const_int;
-  int entries = p.keep;
-  if (p.count != nullptr) entries = min(entries, max(((const_int*)p.count)[id], 0));
-  int len = (int)p.Lk;
-  if (p.k_lens != nullptr) len = min(len, max(((const_int*)p.k_lens)[bk], 0));
+  // what the prologue reads is on its way together: the count and the length, the queries, then the first entries of the list
+  int entries = p.keep, len = (int)p.Lk;
+  if (p.count != nullptr) entries = ((const_int*)p.count)[id];
+  if (p.k_lens != nullptr) len = ((const_int*)p.k_lens)[bk];
+  const int64_t q0 = (int64_t)qb * Q_BLOCK + wave * 64;
+  mfma_bf16x8 qf[4][4];
+#pragma unroll
+  for (int qt = 0; qt < 4; ++qt) {
+    const int64_t r = min(q0 + 16 * qt + n, p.Lq - 1);
+    const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) qf[qt][ks] = *reinterpret_cast<const mfma_bf16x8*>(qp + 32 * ks);
+  }
+  SB();
+  entries = min(p.keep, max(entries, 0));
+  len = min((int)p.Lk, max(len, 0));
   SpList d;
   d.len = uni(len);
   d.nvalid = uni((len + KVBLK - 1) / KVBLK);
@@ -357,7 +370,6 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
   }
   const int nt = d.nvalid > 0 ? uni(e1 - e0) : 0;
 
-  const int64_t q0 = (int64_t)qb * Q_BLOCK + wave * 64;
   SHalf x[2];
   f32x4 negm[4];
 #pragma unroll
@@ -398,26 +410,22 @@ __global__ __launch_bounds__(128, 1) void attn_sparse_kernel(SparseArgs p) {
       m.kofs[i] = (32u * (kt >> 1) + 8u * (r >> 2) + 4u * (kt & 1) + (r & 3u)) * d.rs2 + (((uint32_t)tid & 15u) ^ r) * 16u;
     }
     m.vofs = ((uint32_t)tid >> 3) * m.ldv2 + ((((uint32_t)tid & 7u) ^ (((uint32_t)tid >> 4) & 7u)) << 4);
-    sp_load(d); sp_apply(d);
+    const int first[3] = {d.p[0], d.p[min(1, d.last)], d.p[min(2, d.last)]};
+    d.pos = 3;
+    d.nxt = uni(first[0]); sp_apply(d);
     d.rem0 = d.rem3;
     sp_fetch<0, 0>(m, d);
-    sp_load(d); sp_apply(d);
+    d.nxt = uni(first[1]); sp_apply(d);
     d.rem1 = d.rem3;
     sp_fetch<1, 1>(m, d);
-    sp_load(d); sp_apply(d);
+    d.nxt = uni(first[2]); sp_apply(d);
     d.rem2 = d.rem3;
 
-    mfma_bf16x8 qf[4][4], kf[4][4], vf[8][2];
+    mfma_bf16x8 kf[4][4], vf[8][2];
 #pragma unroll
-    for (int qt = 0; qt < 4; ++qt) {
-      const int64_t r = min(q0 + 16 * qt + n, p.Lq - 1);
-      const bf16_t* qp = p.q + (int64_t)b * p.q_batch + r * p.q_row + (int64_t)h * 128 + g * 8;
+    for (int qt = 0; qt < 4; ++qt)
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        qf[qt][ks] = *reinterpret_cast<const mfma_bf16x8*>(qp + 32 * ks);
-        asm volatile("" : "+a"(qf[qt][ks]));
-      }
-    }
+      for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+a"(qf[qt][ks]));
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
@@ -677,8 +685,8 @@ __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs p, int wgs)
 // How a launch's lists are cut.  Up to 16 queries: one workgroup for every four blocks of a list, up to 1,024 in all.  Else 512 workgroups run at a time, and what is left
 // of the lists behind whole rounds of 512 is cut into the number of shares that takes the least time: what was measured is 1.4 us a block, and for shares 7 us for the join and
 // 0.28 ns for each of a list's rows and shares (its partial sums are written and read), while all of them run at a time.  Lists x blocks, in us whole and in shares:
-// 12 x 100 (64 queries each) 150, in 16 shares 32.8; 64 x 140 209, in 8 60.8, in 4 74; 96 x 32 60.5, in 4 41.6; 96 x 8 24.0, in 2 29.4; 36 x 4 15.7, in 2 17.6;
-// 312 x 48 109, in 2 137; 516 x 64 221, the last four in shares 150; 756 x 64 225 and 206.
+// 12 x 100 (64 queries each) 148, in 16 shares 30.4; 64 x 140 205, in 8 58.1, in 4 70.4; 96 x 32 57.3, in 4 38.1; 96 x 8 22.9, in 2 28.1; 36 x 4 14.4, in 2 16.4;
+// 220 x 48 79.4, in 2 65.2, in 3 86.7; 516 x 64 with the last four in shares 138, at an earlier state 150 where it took 221 uncut; 756 x 64 191, then 206 and 225.
 struct SparsePlan {
   int64_t whole, cut;
   int parts;
