@@ -26,9 +26,9 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
 //   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
 //     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
-// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 11.8 ms, 1.24 PFLOP/s, the matrix pipe busy for about 63 % of the cycles at 1.9 GHz, the waves
-// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 682 us.  (The queries' sixteen loads
-// one behind the other in front of the first tile cost 5 % of that.)
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 11.8 to 12.5 ms by the card, 1.17 to 1.24 PFLOP/s, the matrix pipe busy for about 63 % of the cycles at 1.9 GHz, the waves
+// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 682 to 728 us.  (The queries' sixteen
+// loads one behind the other in front of the first tile cost 1 % of the one and 2 % of the other.)
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
 // MFMA 0); a score is multiplied in the odd gap in front of its exp2, a pair packed in the odd gap behind its second, fragments summed by one MFMA more behind
 // the last product of each; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
