@@ -259,8 +259,9 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
       bias = load_bias((int64_t)at.x * MXM_BN);
     }
 
-    // ---- epilogue: straight from the registers.  Rows past the matrix fall outside the descriptors' num_records; a lane's 8 columns are inside or
-    // outside as a whole (N % 8 == 0), outside: an offset past num_records --------------------------------------------------------------------
+    // ---- epilogue: straight from the registers.  The descriptors end with the tile's last column of the matrix's last row: what a row past the matrix would store
+    // (or read of the residual) begins a whole pitch behind that row's start, and ldc >= N is no less than the tile's columns, however few they are.  A lane's 8
+    // columns are inside or outside as a whole (N % 8 == 0), outside: an offset past num_records ----------------------------------------------------------------
     // (its arguments are read from the kernel's again: held across the loop they take the scalar registers that the streams need)
     typedef __attribute__((address_space(4))) const MxGemm mxm_args;
     mxm_args* pe = (mxm_args*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
     const uint32_t ne = lane_e & 15u, ge = lane_e >> 4;
     const uint32_t colb = (uint32_t)(wx * 128) * 2u + ne * 16u;
     const int64_t rows_valid = min(pe->M - y0, (int64_t)MXM_BM);
-    const uint32_t onum = (uint32_t)((rows_valid - 1) * pe->ldc * 2 + MXM_BN * 2);
+    const uint32_t onum = (uint32_t)((rows_valid - 1) * pe->ldc * 2 + min(pe->N - x0, (int64_t)MXM_BN) * 2);
     const uint32_t ldo2 = (uint32_t)(pe->ldc * 2);
     const __amdgpu_buffer_rsrc_t odesc = __builtin_amdgcn_make_buffer_rsrc((void*)(pe->C + y0 * pe->ldc + x0), 0, (int)onum, 0x00020000);
     const __amdgpu_buffer_rsrc_t rdesc = __builtin_amdgcn_make_buffer_rsrc((void*)((EPI == WAN_EPI_GATE_RES ? pe->R : pe->C) + y0 * pe->ldc + x0), 0, (int)onum, 0x00020000);
