@@ -148,7 +148,8 @@ __global__ __launch_bounds__(512, 4) void conv3d_halo_kernel(HaloP p) {
   int ybase[RT];
 #pragma unroll
   for (int a = 0; a < RT; ++a) ybase[a] = ((RT * wr + a) * HP + n) * HPITCH + lg * 16;   // before the swizzle (it depends on the tap: bit 2 of the patch pixel)
-  const int xbase = HW0 + (wc * NW + n) * 64 + ((lg ^ ((n >> 1) & 2)) << 4);   // (NW is a multiple of 16: bit 2 of the row is bit 2 of n)
+  int xbase = HW0 + (wc * NW + n) * 64 + ((lg ^ ((n >> 1) & 2)) << 4);   // (NW is a multiple of 16: bit 2 of the row is bit 2 of n)
+  asm volatile("" : "+v"(xbase));   // (one register: hipcc keeps its terms apart from the peeled first group to the loop, in scratch with 128 channels)
 
   int kt = 0, cb = 0;                                   // group g
   int kt1 = (G > 1 && p.CB == 1) ? 1 : 0, cb1 = (G > 1 && p.CB > 1) ? 1 : 0;   // group g + 1 (the last group repeats itself: its re-loads land in idle stages)
