@@ -42,7 +42,7 @@ def test_the_library_is_built_without_packed_fp32():
     assert sorted(s[:-4] for s in line.split()) == UNITS                                     # nothing is built otherwise
 
 
-@pytest.mark.parametrize("unit", [u for u in UNITS if u != "gemm256k"])
+@pytest.mark.parametrize("unit", UNITS)
 def test_no_packed_fp32_instruction_and_no_scratch(asm, unit):
     text = asm(unit)
     spilled, packed = {}, set()
@@ -58,7 +58,7 @@ def test_no_packed_fp32_instruction_and_no_scratch(asm, unit):
     assert not spilled and not packed, (spilled, packed)
 
 
-@pytest.mark.parametrize("check", ["test_gemm256k_main_loop_instruction_mix", "test_attention_w64q_no_scratch_and_hardware_conversions",
+@pytest.mark.parametrize("check", ["test_gemm256k_registers_lds_and_no_scratch", "test_gemm256k_main_loop_instruction_mix", "test_attention_w64q_no_scratch_and_hardware_conversions",
                                    "test_attention_bounded_loop_instruction_mix", "test_attention_bounded_tile_scalar_and_wait_instructions", "test_attention_w16n_tile_instruction_mix",
                                    "test_gemm256m_registers_and_stage_instruction_mix", "test_attention_xkv_stream_has_no_valu_write_in_front_of_an_mfma_that_reads_it"])
 def test_hot_kernels_as_they_ship(asm, monkeypatch, check):

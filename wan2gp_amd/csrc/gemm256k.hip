@@ -253,8 +253,13 @@ __global__ __launch_bounds__(256) void gemm256k_kernel(const bf16_t* __restrict_
   asm volatile("" ::: "memory");
   constexpr int EROW = 272;      // bytes per parked row: 256 + 16 (ds_write_b128 of 16 lanes on consecutive rows: 64 banks once)
   char* const park = smem + wave * (128 * EROW);
+  // (the GELU form takes the lane's number afresh: threadIdx.x kept across the K loop for these addresses was one register too many, 8 bytes of scratch.  The gated
+  // form, which holds other things here, has 68 bytes of scratch that way and none with the number kept)
+  int lane_e = lane;
+  if (EPI == WAN_EPI_GELU_TANH) asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_e));
+  const int l31e = lane_e & 31, halfe = lane_e >> 5;
   // read-back geometry: instruction i covers rows 4i .. 4i+3 of the wave's sub-tile, lane -> (row 4i + lane/16, 16-B chunk lane%16)
-  const int prow = lane >> 4, pchunk = lane & 15;
+  const int prow = lane_e >> 4, pchunk = lane_e & 15;
   const int64_t xc = x0 + wx * 128 + pchunk * 8;          // first of the lane's 8 columns: the same for every row group
   const bool col_full = xc + 8 <= XN;
   const int64_t yrow0 = y0 + wy * 128 + prow;
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(256) void gemm256k_kernel(const bf16_t* __restrict_
   };
 #pragma unroll
   for (int xt = 0; xt < 4; ++xt) {
-    const int64_t xb = x0 + wx * 128 + xt * 32 + half * 16;
+    const int64_t xb = x0 + wx * 128 + xt * 32 + halfe * 16;
     float bcol[16];
     if (!BIAS_ROWS) {
 #pragma unroll
@@ -300,7 +305,7 @@ __global__ __launch_bounds__(256) void gemm256k_kernel(const bf16_t* __restrict_
     }
 #pragma unroll
     for (int yt = 0; yt < 4; ++yt) {
-      int64_t yr = y0 + wy * 128 + yt * 32 + l31;
+      int64_t yr = y0 + wy * 128 + yt * 32 + l31e;
       if (yr > YM - 1) yr = YM - 1;
       float v[16];
       const float brow = (BIAS_ROWS && bias != nullptr) ? ld16<F16>(bias[yr]) : 0.f;
@@ -311,7 +316,7 @@ __global__ __launch_bounds__(256) void gemm256k_kernel(const bf16_t* __restrict_
         // nn.Linear output is a 16-bit tensor: GELU sees the rounded value; otherwise the pack below is that rounding
         if (EPI == WAN_EPI_GELU_TANH) v[r] = g256k_gelu_tanh(rnd16<F16>(v[r]));
       }
-      uint4* dst = reinterpret_cast<uint4*>(park + (yt * 32 + l31) * EROW + (xt * 32 + half * 16) * 2);
+      uint4* dst = reinterpret_cast<uint4*>(park + (yt * 32 + l31e) * EROW + (xt * 32 + halfe * 16) * 2);
       dst[0] = pack8t<F16>(v);
       dst[1] = pack8t<F16>(v + 8);
     }
