@@ -480,6 +480,10 @@ def mxfp4_quantize(x):
 
 
 def _mx_operand(codes, scales, name):
+    """(M, K, codes as bytes) of a quantised operand.  Codes that arithmetic has widened (8 * a truth value is int64) still hold a byte each: they are
+    converted, a pass over them in every call."""
+    if codes.dtype != torch.uint8 and codes.is_cuda and codes.dtype in (torch.int8, torch.int16, torch.int32, torch.int64):
+        codes = codes.to(torch.uint8)
     _req(codes, torch.uint8, name); _req(scales, torch.uint8, name + " scales")
     shape = codes.shape
     row = shape[-1] if shape else 0
@@ -491,12 +495,12 @@ def _mx_operand(codes, scales, name):
     need = _L.load().wan_mxfp4_scale_bytes(M, K)
     if scales.numel() != need:
         raise _L.WanHipError(f"{name} scales must hold {need} bytes, got {scales.numel()}")
-    return M, K
+    return M, K, codes
 
 
 def mxfp4_dequantize(codes, scales):
     """The values that mxfp4_quantize's codes stand for, bf16 [..., K] (exact)."""
-    M, K = _mx_operand(codes, scales, "codes")
+    M, K, codes = _mx_operand(codes, scales, "codes")
     out = torch.empty(*codes.shape[:-1], K, dtype=BF16, device=codes.device)
     if M:
         _call(codes.device, _L.load().wan_mxfp4_dequantize, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), M, K)
@@ -506,22 +510,23 @@ def mxfp4_dequantize(codes, scales):
 def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, residual=None, mod=None, e=None, gate_idx=-1, out=None, ldc=None,
                  x_mx=None):
     """nn.Linear on MXFP4 operands with an optional fused epilogue (linear's): x [..., K] bf16 is quantised (or pass x_mx = mxfp4_quantize(x) to share
-    it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight).  out may be the
-    residual, not x."""
+    it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight).  Codes of a wider integer
+    type are converted to bytes in the call.  out may be the residual, not x."""
     for t, n in ((bias, "bias"), (residual, "residual"), (mod, "mod"), (e, "e"), (out, "out")):
         _req(t, BF16, n)
     if weight_codes.dim() != 2:
         raise _L.WanHipError(f"weight_codes must be [N, K / 2], got {list(weight_codes.shape)}")
-    N, K = _mx_operand(weight_codes, weight_scales, "weight_codes")
+    N, K, weight_codes = _mx_operand(weight_codes, weight_scales, "weight_codes")
     if x_mx is None:
         M, Kx, row = _mx_rows(x)
         shape = x.shape[:-1]
     else:
-        M, Kx = _mx_operand(*x_mx, "x_mx")
-        shape = x_mx[0].shape[:-1]
+        x_codes, x_scales = x_mx
+        M, Kx, x_codes = _mx_operand(x_codes, x_scales, "x_mx")
+        shape = x_codes.shape[:-1]
     if Kx != K:
         raise _L.WanHipError(f"x has rows of {Kx} values, the weight of {K}")
-    _same_device(weight_codes, x if x_mx is None else x_mx[0], bias, residual, mod, e, out)
+    _same_device(weight_codes, x if x_mx is None else x_codes, bias, residual, mod, e, out)
     if bias is not None and bias.numel() != N:
         raise _L.WanHipError(f"bias must hold {N} values")
     if epilogue == EPI_TRANSPOSED:
@@ -557,7 +562,7 @@ def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, r
     if x_mx is None:
         _call(weight_codes.device, lib.wan_linear_mxfp4, x.data_ptr(), row, *tail)
     else:
-        _call(weight_codes.device, lib.wan_gemm_mxfp4, x_mx[0].data_ptr(), x_mx[1].data_ptr(), *tail)
+        _call(weight_codes.device, lib.wan_gemm_mxfp4, x_codes.data_ptr(), x_scales.data_ptr(), *tail)
     return out
 
 
