@@ -587,6 +587,17 @@ def pay_attention(qkv_list, dropout_p=0., softmax_scale=None, causal=False, wind
     return o.type(out_dtype)
 
 
+def _heads_side_by_side(t):
+    """[B, L, H, 128] as block_mean and sparse_attention take it: a slice of a fused projection stays where it is, anything else (a [B, H, L, 128] tensor
+    transposed, one row for all tokens) becomes a contiguous copy."""
+    if t.dim() != 4:
+        return t
+    batch, row, head, one = t.stride()
+    L, H = t.shape[1:3]
+    side = one == 1 and (H <= 1 or head == 128) and (L <= 1 or (row >= H * 128 and row % 8 == 0)) and (t.shape[0] <= 1 or batch % 8 == 0) and t.data_ptr() % 16 == 0
+    return t if side else t.clone(memory_format=torch.contiguous_format)
+
+
 def pay_sparse_attention(qkv_list, keep, k_lens=None, recycle_q=False):
     """pay_attention with every block of 128 queries attending only the `keep` blocks of 64 keys whose mean key has the largest product with the block's mean
     query.  Same conventions: q [B,Lq,H,128], k, v [Bk,Lk,Hk,128], the list is consumed, k / v batch 1 is broadcast, the result has q's
@@ -594,7 +605,7 @@ def pay_sparse_attention(qkv_list, keep, k_lens=None, recycle_q=False):
     q, k, v = qkv_list
     qkv_list.clear()
     out_dtype = q.dtype
-    q = q.to(BF16); k = k.to(BF16); v = v.to(BF16).contiguous()
+    q = _heads_side_by_side(q.to(BF16)); k = _heads_side_by_side(k.to(BF16)); v = v.to(BF16).contiguous()
     if k.shape[1] == 0:
         return torch.zeros(q.shape, dtype=out_dtype, device=q.device)
     index, count = select_blocks(block_mean(q, 128), block_mean(k, 64, k_lens), keep, k_lens)
