@@ -265,7 +265,7 @@ def transpose_v(v, ldv=None):
     C = v.numel() // (B * L)
     ldv = ldv or ((L + 63) // 64) * 64
     vt = torch.empty(B, C, ldv, dtype=BF16, device=v.device)
-    check(_L.load().wan_transpose_v(ptr(v), ptr(vt), B, L, ldv, C, stream_ptr()), "wan_transpose_v")
+    _call(v.device, _L.load().wan_transpose_v, ptr(v), ptr(vt), B, L, ldv, C)
     return vt
 
 
