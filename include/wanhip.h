@@ -159,7 +159,7 @@ int wan_fp8_quantize_pre(const wan_bf16* x, uint8_t* out, float* ws, int64_t n, 
  * wan_gemm_mxfp4: C = epilogue(A W^T + bias), A [M, K] and W [N, K] quantised, C bf16; epilogues and their arguments as wan_gemm_bf16 (the
  *   transposed form writes Ct [N, ldc]).  K % 32 == 0, any M and N.  The whole epilogue in fp32, ONE rounding to bf16 at its end (no
  *   reference plan fixes roundings in between, and each would cost a bit).  scratch: wan_gemm_mxfp4_scratch_bytes(M, N, K) bytes of device memory, 16-byte aligned
- *   (NULL where that is 0); a call overwrites it, calls on different streams must not share it. */
+ *   (NULL where that is 0); a call overwrites it, calls on different streams must not share it.  C may be R; it overlaps no other operand, nor R in part. */
 int64_t wan_mxfp4_scale_bytes(int64_t rows, int64_t K);
 int wan_mxfp4_quantize(const wan_bf16* x, int64_t row_stride, uint8_t* codes, uint8_t* scales, int64_t M, int K, void* stream);
 int wan_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, wan_bf16* out, int64_t M, int K, void* stream);
@@ -169,7 +169,7 @@ int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, 
                    const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes,
                    void* stream);
 /* wan_mxfp4_quantize of x [M, K] bf16 (rows x_row elements apart) into the scratch, then wan_gemm_mxfp4: one call for a Linear whose
- * quantised input nobody else reads.  C must not overlap x (it may be R). */
+ * quantised input nobody else reads.  C must not overlap x either. */
 int64_t wan_linear_mxfp4_scratch_bytes(int64_t M, int N, int K);
 int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C,
                      int64_t ldc, int64_t M, int N, int K, int epilogue, const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e,

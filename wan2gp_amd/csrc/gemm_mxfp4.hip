@@ -443,6 +443,22 @@ extern "C" int64_t wan_gemm_mxfp4_scratch_bytes(int64_t M, int N, int K) {
   return parts <= 1 ? 0 : (int64_t)parts * M * N * 4;
 }
 
+// Whether the output shares memory with x: workgroups may read x while others already write.  (Rows side by side in one buffer share a range, but no element.)
+static bool mx_overlaps(const wan_bf16* x, int64_t x_row, const wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue) {
+  const bool tr = epilogue == WAN_EPI_TRANSPOSED;
+  const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((M - 1) * x_row + K) * 2, c0 = (uintptr_t)C, c1 = c0 + ((tr ? N - 1 : M - 1) * ldc + (tr ? M : N)) * 2;
+  if (x1 <= c0 || c1 <= x0) return false;
+  if (tr || x_row != ldc || M == 1) return true;
+  const int64_t d = ((int64_t)(c0 / 2) - (int64_t)(x0 / 2)) % ldc, at = d < 0 ? d + ldc : d;   // C's first column, counted from x's
+  return !(at >= K && at + N <= ldc);
+}
+// ... and with one of the small operands, or the weights
+static bool mx_touches(const wan_bf16* C, int64_t ldc, int64_t M, int N, int epilogue, const void* p, int64_t bytes) {
+  const bool tr = epilogue == WAN_EPI_TRANSPOSED;
+  const uintptr_t c0 = (uintptr_t)C, c1 = c0 + ((tr ? N - 1 : M - 1) * ldc + (tr ? M : N)) * 2, p0 = (uintptr_t)p;
+  return p != nullptr && p0 < c1 && c0 < p0 + bytes;
+}
+
 static int mx_gemm_check(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue,
                          const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch) {
   WAN_REQUIRE(A && a_scales && W && w_scales && C, "wan_gemm_mxfp4: null operand");
@@ -459,6 +475,20 @@ static int mx_gemm_check(const uint8_t* A, const uint8_t* a_scales, const uint8_
   return 0;
 }
 
+// One workgroup's output would be another's operand.  (A residual that is the output itself is read by the lane alone that writes its place.)
+static int mx_gemm_aliases(const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, const wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue, const wan_bf16* R,
+                           const wan_bf16* mod, const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch) {
+  WAN_REQUIRE(!mx_touches(C, ldc, M, N, epilogue, W, (int64_t)N * (K / 2)) && !mx_touches(C, ldc, M, N, epilogue, w_scales, wan_mxfp4_scale_bytes(N, K)) &&
+                  !mx_touches(C, ldc, M, N, epilogue, bias, (int64_t)N * 2),
+              "wan_gemm_mxfp4: the output must not overlap the weights or the bias");
+  if (epilogue != WAN_EPI_GATE_RES) return 0;
+  WAN_REQUIRE(R == C || !mx_overlaps(R, ldc, C, ldc, M, N, N, epilogue), "wan_gemm_mxfp4: an output that overlaps the residual must be the residual");
+  WAN_REQUIRE(gate_idx < 0 || (!mx_touches(C, ldc, M, N, epilogue, mod, (int64_t)n_mod * N * 2) &&
+                               !mx_touches(C, ldc, M, N, epilogue, e, (M + rows_per_batch - 1) / rows_per_batch * n_mod * N * 2)),
+              "wan_gemm_mxfp4: the output must not overlap the gate");
+  return 0;
+}
+
 extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const uint8_t* W, const uint8_t* w_scales, const wan_bf16* bias, wan_bf16* C, int64_t ldc, int64_t M, int N, int K,
                               int epilogue, const wan_bf16* R, const wan_bf16* mod, const wan_bf16* e, int n_mod, int gate_idx, int64_t rows_per_batch, void* scratch, int64_t scratch_bytes,
                               void* stream) {
@@ -466,6 +496,10 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
   if (bad != 0) return bad;
   const int64_t need = wan_gemm_mxfp4_scratch_bytes(M, N, K);
   WAN_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0), "wan_gemm_mxfp4: needs 16-byte aligned scratch of %lld bytes", (long long)need);
+  const int alias = mx_gemm_aliases(W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
+  if (alias != 0) return alias;
+  WAN_REQUIRE(!mx_touches(C, ldc, M, N, epilogue, A, M * (K / 2)) && !mx_touches(C, ldc, M, N, epilogue, a_scales, wan_mxfp4_scale_bytes(M, K)),
+              "wan_gemm_mxfp4: the output must not overlap the quantised rows");
   const bool tr = epilogue == WAN_EPI_TRANSPOSED;
   hipStream_t st = as_stream(stream);
   const MxGemm p = {tr ? W : A, tr ? w_scales : a_scales, tr ? A : W, tr ? a_scales : w_scales, tr ? N : M, tr ? M : N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx,
@@ -483,16 +517,6 @@ extern "C" int wan_gemm_mxfp4(const uint8_t* A, const uint8_t* a_scales, const u
     case WAN_EPI_GATE_RES: return mxg_launch<WAN_EPI_GATE_RES>(p, plan, ws, st);
     default: return mxg_launch<WAN_EPI_TRANSPOSED>(p, plan, ws, st);
   }
-}
-
-// Whether the output shares memory with x: workgroups may read x while others already write.  (Rows side by side in one buffer share a range, but no element.)
-static bool mx_overlaps(const wan_bf16* x, int64_t x_row, const wan_bf16* C, int64_t ldc, int64_t M, int N, int K, int epilogue) {
-  const bool tr = epilogue == WAN_EPI_TRANSPOSED;
-  const uintptr_t x0 = (uintptr_t)x, x1 = x0 + ((M - 1) * x_row + K) * 2, c0 = (uintptr_t)C, c1 = c0 + ((tr ? N - 1 : M - 1) * ldc + (tr ? M : N)) * 2;
-  if (x1 <= c0 || c1 <= x0) return false;
-  if (tr || x_row != ldc || M == 1) return true;
-  const int64_t d = ((int64_t)(c0 / 2) - (int64_t)(x0 / 2)) % ldc, at = d < 0 ? d + ldc : d;   // C's first column, counted from x's
-  return !(at >= K && at + N <= ldc);
 }
 
 // the quantised rows and their scales in front of the product's own scratch
@@ -514,6 +538,8 @@ extern "C" int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t*
     const int rc = mx_gemm_check(some, some, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
     if (rc != 0) return rc;
     WAN_REQUIRE(!mx_overlaps(x, x_row, C, ldc, M, N, K, epilogue), "wan_linear_mxfp4: the output must not overlap x");
+    const int alias = mx_gemm_aliases(W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
+    if (alias != 0) return alias;
     const MxGemm p = {nullptr, nullptr, nullptr, nullptr, M, N, K, (K + 255) / 256, bias, C, ldc, R, mod, e, n_mod, gate_idx, rows_per_batch > 0 ? rows_per_batch : 1};
     return mxr_launch(x, x_row, nullptr, nullptr, W, w_scales, M, N, p, epilogue, as_stream(stream));
   }
@@ -526,6 +552,8 @@ extern "C" int wan_linear_mxfp4(const wan_bf16* x, int64_t x_row, const uint8_t*
   const int rc = mx_gemm_check(codes, scales, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
   if (rc != 0) return rc;
   WAN_REQUIRE(!mx_overlaps(x, x_row, C, ldc, M, N, K, epilogue), "wan_linear_mxfp4: the output must not overlap x");
+  const int alias = mx_gemm_aliases(W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch);
+  if (alias != 0) return alias;
   const int rq = wan_mxfp4_quantize(x, x_row, codes, scales, M, K, stream);
   if (rq != 0) return rq;
   return wan_gemm_mxfp4(codes, scales, W, w_scales, bias, C, ldc, M, N, K, epilogue, R, mod, e, n_mod, gate_idx, rows_per_batch, rest, scratch_bytes - (rest - codes), stream);
