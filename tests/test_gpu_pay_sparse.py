@@ -49,3 +49,25 @@ def test_one_row_for_all(ops):
         assert torch.equal(ops.pay_sparse_attention([view, k, v], 2), ops.pay_sparse_attention([view.contiguous(), k, v], 2))
     for view in (k[:, :1].expand(-1, 300, -1, -1), k[:, :, :1].expand(-1, -1, 4, -1), k[:1].expand(2, -1, -1, -1)):
         assert torch.equal(ops.pay_sparse_attention([q, view, v], 2), ops.pay_sparse_attention([q, view.contiguous(), v], 2))
+
+
+@pytest.mark.parametrize("B,Lq,Lk", [(0, 200, 300), (2, 0, 300), (2, 200, 0), (0, 0, 0)])
+def test_nothing_to_attend(ops, B, Lq, Lk):
+    q, k, v = rnd(7, B, Lq, 2, 128), rnd(8, B, Lk, 2, 128), rnd(9, B, Lk, 2, 128)
+    qm, km = ops.block_mean(q, 128), ops.block_mean(k, 64)
+    index, count = ops.select_blocks(qm, km, 3)
+    assert index.shape == (B, 2, (Lq + 127) // 128, 3) and count.shape == index.shape[:3]
+    if Lk == 0:
+        assert (index == -1).all() and (count == 0).all()
+    o = ops.pay_sparse_attention([q, k, v], 3)
+    assert o.shape == q.shape and o.dtype == BF and (o == 0).all()
+
+
+@pytest.mark.parametrize("keep", [0, -1])
+def test_no_blocks_to_keep_is_refused(ops, keep):
+    from wan2gp_amd.lib import WanHipError
+    q = rnd(10, 1, 200, 2, 128)
+    with pytest.raises(WanHipError, match="keep"):
+        ops.select_blocks(ops.block_mean(q, 128), ops.block_mean(q, 64), keep)
+    with pytest.raises(WanHipError, match="keep"):
+        ops.pay_sparse_attention([q, q, q], keep)

@@ -401,12 +401,14 @@ def select_blocks(q_mean, k_mean, keep, k_lens=None):
     Bk, Hk, nk, _ = k_mean.shape
     _same_device(q_mean, k_mean)
     _lens(k_lens, Bk, "k_lens", q_mean.device)
+    if keep < 1:
+        raise _L.WanHipError(f"keep must be positive, got {keep}")
     index = torch.empty(B, H, nq, keep, dtype=torch.int32, device=q_mean.device)
     count = torch.empty(B, H, nq, dtype=torch.int32, device=q_mean.device)
-    if nk == 0 and k_mean.shape[0] and keep > 0:
-        return index.fill_(-1), count.zero_()
-    if nq == 0 and B and H and keep > 0:
+    if q_mean.numel() == 0:
         return index, count
+    if nk == 0 and Bk:
+        return index.fill_(-1), count.zero_()
     lib = _L.load()
     need = int(lib.wan_select_blocks_scratch_bytes(B, H, nq, nk))
     ws = torch.empty(need, dtype=torch.uint8, device=q_mean.device) if need else None
@@ -606,7 +608,7 @@ def pay_sparse_attention(qkv_list, keep, k_lens=None, recycle_q=False):
     qkv_list.clear()
     out_dtype = q.dtype
     q = _heads_side_by_side(q.to(BF16)); k = _heads_side_by_side(k.to(BF16)); v = v.to(BF16).contiguous()
-    if k.shape[1] == 0:
+    if q.numel() == 0 or k.shape[1] == 0:
         return torch.zeros(q.shape, dtype=out_dtype, device=q.device)
     index, count = select_blocks(block_mean(q, 128), block_mean(k, 64, k_lens), keep, k_lens)
     own = q.is_contiguous() and q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr()
