@@ -25,8 +25,9 @@ SHORT = {"v_exp_f32_e32": "EXP", "v_add_f32": "ADD", "v_cvt_pk_bf16_f32": "CVT",
 def asm_of(unit, defines):
     out = os.path.join(tempfile.mkdtemp(prefix="isa_"), unit + ".s")
     src = os.path.join(ROOT, "wan2gp_amd", "csrc", unit + ".hip")
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-function", "-ffp-contract=on",
-                    "-I" + os.path.join(ROOT, "include"), *defines, "-S", "--cuda-device-only", src, "-o", out], check=True,
+    line = re.search(r"^CXXFLAGS = (.*)$", open(os.path.join(ROOT, "wan2gp_amd", "csrc", "Makefile")).read(), re.M).group(1)   # what the library is built with
+    flags = line.replace("$(ARCH)", "gfx950").replace("$(EXTRA)", "").split()
+    subprocess.run(["/opt/rocm/bin/hipcc", *flags, "-I" + os.path.join(ROOT, "include"), *defines, "-S", "--cuda-device-only", src, "-o", out], check=True,
                    stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
     return open(out).read()
 

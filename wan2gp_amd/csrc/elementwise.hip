@@ -43,19 +43,15 @@ __device__ __forceinline__ void load_row(uint4 (&r)[NCH], const bf16_t* x, int l
 }
 
 // x0' = x0*cos0 - x1*sin0 ; x1' = x1*cos1 + x0*sin1 -- fp32, the four products rounded SEPARATELY (posemb_layers.py:251-267: no fused
-// multiply-add), one bf16 rounding by the caller.  The pair-wise form of rounds 3-5: only diagnostics builds (ROPE_FORM 0 / 2) call it.
+// multiply-add), one bf16 rounding by the caller.  The pair-wise form: only diagnostics builds (ROPE_FORM 0) call it.
 __device__ __forceinline__ wan_f32x2 rope_pair(wan_f32x2 y, float c0, float c1, float s0, float s1) {
 #pragma clang fp contract(off)
   const wan_f32x2 cc = {c0, c1};
   const wan_f32x2 ss = {-s0, s1};
   const wan_f32x2 p = y * cc;
-#if ROPE_FORM == 2     // diagnostics: the packed crosswise multiply, but never onto its own source pair
-  wan_f32x2 q;
-  asm volatile("v_pk_mul_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[1,0]" : "=&v"(q) : "v"(ss), "v"(y));
-#else                  // hipcc fuses this into v_pk_mul_f32 ... op_sel:[0,1] op_sel_hi:[1,0]
+  // (where packing is allowed, hipcc fuses this into v_pk_mul_f32 ... op_sel:[0,1] op_sel_hi:[1,0])
   const wan_f32x2 ys = {y.y, y.x};
   const wan_f32x2 q = ys * ss;      // (-x1*sin0, x0*sin1): the sign flip of a product is exact
-#endif
   return p + q;
 }
 
@@ -170,19 +166,18 @@ __global__ __launch_bounds__(256, (PERSIST && FULL && NCH <= 10 ? (SCATTER ? 2 :
         if (i + 1 < NCH && (FULL || c + 64 < nchunk)) wnext = wlds[c + 64];
       }
       if (FULL || c < nchunk) {
-        // Pairs of elements all the way (round 3): the two bf16 of a 32-bit word stay together through both roundings, the rotation and
-        // the pack, so that every multiply / add is ONE packed-f32 instruction per pair and every rounding one v_cvt_pk_bf16_f32 per
-        // pair (the scalar form rounded with cvt_pk(f, 0): 144 VALU instructions per 16-byte chunk, this form ~90).  Same operations
-        // per element in the same order: bit-identical results (tests/test_gpu_ops.py).
+        // Pairs of elements all the way: the two bf16 of a 32-bit word stay together through both roundings, the rotation and
+        // the pack, so that every rounding is one v_cvt_pk_bf16_f32 per pair (the scalar form rounded with cvt_pk(f, 0)).  Multiplies and adds are one
+        // instruction an element (common.h: no packed fp32).  Same operations per element in the same order: bit-identical results (tests/test_gpu_ops.py).
         const uint4 wraw = PERSIST ? wcur : *reinterpret_cast<const uint4*>(w + c * 8);
         const uint32_t ww[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
         const uint32_t vw[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         uint32_t ow[4];
 #if ROPE_FORM == 1
-        // Two words (= two rotation pairs A, B) at a time, as E = (x0 of A, x0 of B) and O = (x1 of A, x1 of B): every multiply and add of the
-        // row is then a packed-f32 instruction on ALIGNED register pairs -- x0' = E C0 + O (-S0), x1' = O C1 + E S1 -- where the pair-wise form
-        // (rounds 3-5, below) needed (-x1 sin0, x0 sin1): v_pk_mul_f32 ... op_sel:[0,1] op_sel_hi:[1,0], the instruction that lost its low product
-        // beside a neighbour process (common.h).  Same operations per element, same roundings: identical bytes (tools/rows_hash.py).
+        // Two words (= two rotation pairs A, B) at a time, as E = (x0 of A, x0 of B) and O = (x1 of A, x1 of B): x0' = E C0 + O (-S0), x1' = O C1 + E S1,
+        // on ALIGNED register pairs even where packing is allowed -- the pair-wise form (below) then needs (-x1 sin0, x0 sin1): v_pk_mul_f32 ...
+        // op_sel:[0,1] op_sel_hi:[1,0], the instruction that lost its low product beside a neighbour process (common.h).  Same operations per element,
+        // same roundings: identical bytes (tools/rows_hash.py).
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma clang fp contract(off)
@@ -207,7 +202,7 @@ __global__ __launch_bounds__(256, (PERSIST && FULL && NCH <= 10 ? (SCATTER ? 2 :
           E = E * oscale; O = O * oscale;                              // (x * 1.0f is x: no select on a launch constant inside the row)
           ow[2 * h] = pack2bf(E.x, O.x); ow[2 * h + 1] = pack2bf(E.y, O.y);
         }
-#else   // ROPE_FORM 0 / 2: the pair-wise form of rounds 3-5 (diagnostics, `make rrwg`)
+#else   // ROPE_FORM 0: the pair-wise form (diagnostics, `make rrwg`)
 #pragma unroll
         for (int pq = 0; pq < 4; ++pq) {
           wan_f32x2 v2 = {__uint_as_float(vw[pq] << 16), __uint_as_float(vw[pq] & 0xffff0000u)};
@@ -467,7 +462,7 @@ __global__ __launch_bounds__(256) void nag_combine_kernel(const bf16_t* x_pos, c
 // ------------------------------------------------------------------------------------------------
 __global__ void sinusoid_kernel(const float* __restrict__ t, bf16_t* __restrict__ out, int n, int dim) {
   // cat([cos(t * 10000^(-i/half)), sin(...)])   model.py:32-42
-  wan_hold_lds_word();   // (common.h: cosf / sinf hold packed instructions that read a register pair crosswise)
+  wan_hold_lds_word();   // (common.h)
   const int half = dim / 2;
   const int idx = blockIdx.x * blockDim.x + threadIdx.x;
   if (idx >= n * half) return;
