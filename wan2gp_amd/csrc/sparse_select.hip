@@ -233,7 +233,8 @@ __global__ __launch_bounds__(512) void block_choose_kernel(const float* __restri
 }
 
 // Up to 2,048: one wave per row, its keys from memory.  Bound by the ballots and the scores' bytes: 23,640 rows of 1,182 in 60 us.  The whole choice took 236 us so and 390 us with
-// the search by a workgroup below; 609 against 937 us at 1,024 x 2,048.
+// the search by a workgroup below; 609 against 937 us at 1,024 x 2,048.  N, the keys a lane holds, goes by the blocks of keys in steps of four: a step is 5 to 8 us of these
+// rows (40 x 591 with 32 keys a lane 359 us in all, with 24 for 1,400 blocks 258, where 32 took 288; 16 for 800 blocks 152, where 19 took 158; 20 for 1,216 blocks 216, 19 213).
 template <int N>
 __global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
                                                                int* __restrict__ count, int H, int Bk, int nq, int nk, int keep, int64_t rows) {
@@ -352,12 +353,19 @@ extern "C" int wan_select_blocks(const float* q_mean, const float* k_mean, const
   const int64_t rows = (int64_t)B * H * nq;
   const dim3 grid((unsigned)((rows + 3) / 4)), wg(256);
 #define SELECT(N) hipLaunchKernelGGL(block_select_wave_kernel<N>, grid, wg, 0, st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep, rows)
-  if (nk <= 640) SELECT(10);
-  else if (nk <= 1216) SELECT(19);
-  else if (nk <= 2048) SELECT(32);
+  switch (nk <= 2048 ? (nk + 255) / 256 : 0) {
+    case 2: SELECT(8); break;
+    case 3: SELECT(12); break;
+    case 4: SELECT(16); break;
+    case 5: SELECT(20); break;
+    case 6: SELECT(24); break;
+    case 7: SELECT(28); break;
+    case 8: SELECT(32); break;
 #undef SELECT
-  else if (nk <= 6800) hipLaunchKernelGGL(block_select_kernel<4>, dim3((unsigned)rows), wg, (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
-  else hipLaunchKernelGGL(block_select_kernel<16>, dim3((unsigned)rows), dim3(1024), (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+    default:
+      if (nk <= 6800) hipLaunchKernelGGL(block_select_kernel<4>, dim3((unsigned)rows), wg, (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+      else hipLaunchKernelGGL(block_select_kernel<16>, dim3((unsigned)rows), dim3(1024), (unsigned)(nk * 8), st, keys, k_lens, index, count, H, Bk, (int)nq, (int)nk, keep);
+  }
   WAN_LAUNCH_CHECK();
   return 0;
 }
