@@ -26,9 +26,11 @@ constexpr float SPARSE_SCALE_LOG2E = 0.08838834764831845f * 1.4426950408889634f;
 //     above the row's reference, the first tile and tiles that end inside leave the straight path (sp_cold).
 //   * q is not scaled in front: rounded with the scale in it every score would be off by 2^-9 of its terms (outputs 0.0028 from the exact ones where now it is
 //     0.0023, and the rounding of the outputs alone 0.0017).  The multiplication per score costs 4 % of a large call.
-// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 11.8 to 12.5 ms by the card, 1.17 to 1.24 PFLOP/s, the matrix pipe busy for about 63 % of the cycles at 1.9 GHz, the waves
-// waiting for the next instruction's slot or the DMA's landing for a sixth each.  32,760 tokens of 12 heads, 64 blocks: 682 to 728 us.  (The queries' sixteen
-// loads one behind the other in front of the first tile cost 1 % of the one and 2 % of the other.)
+//   * the weights are rounded to bf16 (2^-8 each), which is what the product with V takes, and summed so rounded.  Two terms, the second what the first leaves, would
+//     bring the outputs to their own rounding for half as many MFMAs again, and make NaN of an infinity in V (times a second term of 0 or less) where one term keeps it.
+// Bound inside the CU: 75,600 tokens of 40 heads with 148 of 1,182 blocks each in 11.8 to 13.1 ms by the card, 1.12 to 1.24 PFLOP/s, the matrix pipe busy for 64 % of the cycles (1.77 GHz in
+// the counters' run).  32,760 tokens of 12 heads, 64 blocks: 682 to 738 us, 59 %.  (The queries' sixteen loads one behind the other in front of the first tile cost
+// 1 % of the one and 2 % of the other.)
 // Gap plan (even gaps: one exp2 each): exp2 of a's score k behind MFMA 52 + 2 k, of b's behind 116 + 2 k, running into the next tile (k = 6 behind its
 // MFMA 0); a score is multiplied in the odd gap in front of its exp2, a pair packed in the odd gap behind its second, fragments summed by one MFMA more behind
 // the last product of each; maxima of a in the odd gaps 29 .. 51, of b 93 .. 115; DMA of tile
@@ -619,7 +621,7 @@ __global__ __launch_bounds__(256) void attn_sparse_few_kernel(SparseArgs p) {
         w[j] = __builtin_amdgcn_exp2f(s[2 * c + (j >> 2)][j & 3] - ref);
         l += w[j];
       }
-      const mfma_bf16x8 pk = __builtin_bit_cast(mfma_bf16x8, pack8(w));
+      const mfma_bf16x8 pk = __builtin_bit_cast(mfma_bf16x8, pack8(w));   // (one bf16 term as above; the row sum takes the weights as they are)
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[dt][c], pk, acc[dt], 0, 0, 0);
     }

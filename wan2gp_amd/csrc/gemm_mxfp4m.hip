@@ -16,9 +16,9 @@
 //   * K need not be a multiple of 256: what a row's last stage reads past the row is the next row's codes (the buffer's end reads as zeros), and the
 //     scale bytes there are 0 on both sides -- (6 * 2^-127)^2 is 0 in fp32.
 //   * stores are non-temporal: 256 tiles are 32 MB, more than the L2 keeps for whoever reads them (with ordinary stores 5 % slower).
-// Bound by the card's power where K is long: 75,600 x 5,120 x 13,824 with the gated residual in 2.17 - 2.30 ms by the card, 4.7 - 4.9 PFLOP/s, 67 % of the cycles on the matrix pipe
-// at 1.4 GHz; the same MFMAs with no memory access between them would take 1.75 ms.  Where K is short, by the epilogue: at K = 1,536 the GELU's
-// 48 VALU cycles an element are as much as the products' (292 us, 3.1 PFLOP/s).
+// Bound by the card's power where K is long: 75,600 x 5,120 x 13,824 with the gated residual in 2.15 - 2.30 ms by the card, 4.7 - 5.0 PFLOP/s, 66 % of the cycles on the matrix pipe
+// (1.6 GHz in the counters' run); a bare stream of these MFMAs on normally distributed blocks runs at 6.97 PFLOP/s (8.92 on zeros: the operands' power), 1.54 ms.  Where K is short, by the epilogue: at K = 1,536 the GELU's
+// 48 VALU cycles an element are as much as the products' (290 us, 3.1 PFLOP/s, 37 % of the cycles on the matrix pipe).
 #include "mxfp4.h"
 
 #include <type_traits>
@@ -357,7 +357,9 @@ __global__ __launch_bounds__(256) void gemm_mxfp4m_kernel(MxGemm p, int tiles_y,
 
 // -1: the problem does not fit this kernel (gemm_mxfp4.hip's takes it)
 int wan_gemm_mxfp4m_try(const MxGemm& p, int epilogue, hipStream_t st) {
-  if (p.N % 8 != 0 || p.ldc % 8 != 0) return -1;   // a lane stores 8 columns or none
+  // A lane stores 8 columns or none; what the transposed form would store past the tokens lies in the caller's padding, which stays as it was.  So tokens that are no multiple of
+  // 8 take the 128-row tiles: V^T of 75,600 and 75,597 tokens x 5,120 x 5,120 945 and 1,950 us, of 32,760 and 32,757 x 1,536 x 1,536 50 and 131.
+  if (p.N % 8 != 0 || p.ldc % 8 != 0) return -1;
   if (((uintptr_t)p.C | (uintptr_t)p.R | (uintptr_t)p.mod | (uintptr_t)p.e) & 15) return -1;
   if (epilogue != WAN_EPI_TRANSPOSED && ((uintptr_t)p.bias & 15)) return -1;
   if (epilogue == WAN_EPI_GATE_RES && p.gate_idx >= 0 && p.rows_per_batch < MXM_BM) return -1;
