@@ -1,4 +1,4 @@
-"""The transposed epilogue of the scaled-fp8 Linear where a row of the output holds fewer than 256 tokens: exact results (small whole numbers), and nothing in
+"""The transposed epilogue of the bf16 and of the scaled-fp8 Linears where a row of the output holds fewer than 256 tokens: exact results (small whole numbers), and nothing in
 front of the output, behind it or between tokens and ldc touched."""
 import pytest
 import torch
@@ -30,6 +30,15 @@ def guarded(N, ldc):
 def held(buf, out, M, ref):
     assert torch.equal(out[:, :M], ref)
     assert (buf[:GUARD] == 7).all() and (buf[GUARD + len(out):] == 7).all() and (buf[:, M:] == 7).all()
+
+
+@pytest.mark.parametrize("M,N,K,ldc", [(104, 40000, 64, 128), (64, 33000, 128, 64), (248, 20600, 64, 248), (8, 40010, 64, 64), (200, 70001, 128, 200), (130, 30000, 64, 192), (512, 20600, 64, 512),
+                                       (104, 300, 64, 128), (64, 384, 128, 64)])
+def test_bf16(ops, M, N, K, ldc):
+    x, w, b = operands(M, N, K)
+    buf, out = guarded(N, ldc)
+    ops.linear(x, w, b, epilogue=ops.EPI_TRANSPOSED, out=out, ldc=ldc)
+    held(buf, out, M, (w.float() @ x.float().t() + b.float()[:, None]).to(BF))
 
 
 @pytest.mark.parametrize("vector", [False, True])

@@ -360,7 +360,8 @@ __global__ __launch_bounds__(256) void gemm256m_kernel(const bf16_t* __restrict_
     const uint32_t colb = (uint32_t)(wx * 128) * 2u + ne * 16u;  // byte offset of the lane's 8 columns in the tile row
     int64_t rows_valid = YM - y0;
     if (rows_valid > BMY) rows_valid = BMY;
-    const uint32_t onum = (uint32_t)((rows_valid - 1) * ldo * 2 + M_BN * 2);  // rows >= rows_valid: out of range
+    // the end of the last row's columns: a row past the matrix begins behind it however short the rows are (ldo >= XN)
+    const uint32_t onum = (uint32_t)((rows_valid - 1) * ldo * 2 + (BIAS_ROWS ? min(XN - x0, (int64_t)M_BN) : (int64_t)M_BN) * 2);
     const uint32_t ldo2 = (uint32_t)(ldo * 2);
     const __amdgpu_buffer_rsrc_t odesc = __builtin_amdgcn_make_buffer_rsrc((void*)(Out + y0 * ldo + x0), 0, (int)onum, 0x00020000);
     const __amdgpu_buffer_rsrc_t rdesc =
