@@ -233,8 +233,8 @@ __global__ __launch_bounds__(512) void block_choose_kernel(const float* __restri
 }
 
 // Up to 2,048: one wave per row, its keys from memory.  Bound by the ballots and the scores' bytes: 23,640 rows of 1,182 in 62 us.  The whole choice took 237 us so and 390 us with
-// the search by a workgroup below; 609 against 937 us at 1,024 x 2,048.  N, the keys a lane holds, goes by the blocks of keys in steps of four: a step is 5 to 8 us of these
-// rows (40 x 591 with 32 keys a lane 359 us in all, with 24 for 1,400 blocks 258, where 32 took 288; 16 for 800 blocks 152, where 19 took 158; 20 for 1,216 blocks 216, 19 213).
+// the search by a workgroup below; 609 against 937 us at 1,024 x 2,048.  N, the keys a lane holds, goes by the blocks of keys in steps of four: a step is 8 to 15 us of
+// 40 x 591 rows (the whole choice out of 1,400 blocks 258 us with 24 keys a lane, 288 with 32; out of 800 152 with 16, 158 with 19; out of 1,216 216 with 20, 213 with 19).
 template <int N>
 __global__ __launch_bounds__(256) void block_select_wave_kernel(const uint64_t* __restrict__ keys, const int* __restrict__ k_lens, int* __restrict__ index,
                                                                int* __restrict__ count, int H, int Bk, int nq, int nk, int keep, int64_t rows) {
