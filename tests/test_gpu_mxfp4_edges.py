@@ -98,3 +98,21 @@ def test_rows_further_apart_than_they_are_long(ops, M, N, K, ldc):
                                    ws.data_ptr(), need, lib.stream_ptr()), "wan_gemm_mxfp4")
         ref = (r.float() + y * (mod[3].float() + 1)).to(BF) if epi == lib.EPI_GATE_RES else y.to(BF)
         assert torch.equal(out[:, :N], ref) and (out[:, N:] == 7).all()
+
+
+@pytest.mark.parametrize("M,N,K,shape", [(300, 520, 512, (520, 384)), (104, 256, 64, (1, 256, 256)), (20, 72, 96, (72, 20)), (9000, 1160, 256, (2, 580, 9000))])
+def test_a_transposed_output_is_written_by_its_own_rows(ops, M, N, K, shape):
+    x, w, b, _, _, y = whole(M, N, K)
+    out = torch.full(shape, 7.0, dtype=BF, device="cuda")
+    assert ops.linear_mxfp4(x, *ops.mxfp4_quantize(w), b, epilogue=ops.EPI_TRANSPOSED, out=out) is out
+    rows = out.view(N, -1)
+    assert torch.equal(rows[:, :M], y.to(BF).t()) and (rows[:, M:] == 7).all()
+
+
+def test_a_transposed_output_that_is_too_small_is_refused(ops):
+    from wan2gp_amd.lib import WanHipError
+    x, w, b, _, _, _ = whole(100, 64, 64)
+    wm = ops.mxfp4_quantize(w)
+    for out, ldc in ((torch.zeros(64, 96, dtype=BF, device="cuda"), None), (torch.zeros(63, 128, dtype=BF, device="cuda"), None), (torch.zeros(64, 128, dtype=BF, device="cuda"), 96)):
+        with pytest.raises(WanHipError, match="does not hold"):
+            ops.linear_mxfp4(x, *wm, b, epilogue=ops.EPI_TRANSPOSED, out=out, ldc=ldc)

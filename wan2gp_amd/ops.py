@@ -513,7 +513,8 @@ def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, r
                  x_mx=None):
     """nn.Linear on MXFP4 operands with an optional fused epilogue (linear's): x [..., K] bf16 is quantised (or pass x_mx = mxfp4_quantize(x) to share
     it between Linears of the same input; x may then be None), (weight_codes [N, K/2], weight_scales) = mxfp4_quantize(weight).  Codes of a wider integer
-    type are converted to bytes in the call.  out may be the residual, not x."""
+    type are converted to bytes in the call.  out may be the residual, not x; a transposed result (ldc apart, by default the next multiple of 64) goes
+    into an out of rows by their own length."""
     for t, n in ((bias, "bias"), (residual, "residual"), (mod, "mod"), (e, "e"), (out, "out")):
         _req(t, BF16, n)
     if weight_codes.dim() != 2:
@@ -532,7 +533,7 @@ def linear_mxfp4(x, weight_codes, weight_scales, bias=None, epilogue=EPI_NONE, r
     if bias is not None and bias.numel() != N:
         raise _L.WanHipError(f"bias must hold {N} values")
     if epilogue == EPI_TRANSPOSED:
-        ldc = ldc or ((M + 63) // 64) * 64
+        ldc = ldc or (out.shape[-1] if out is not None and out.dim() > 1 else ((M + 63) // 64) * 64)
         if out is None:
             out = torch.zeros(N, ldc, dtype=BF16, device=weight_codes.device)
         if out.numel() < N * ldc or ldc < M:
